@@ -50,7 +50,8 @@ typedef enum {
   NTB_F16 = 6,
   NTB_BF16 = 7,
   NTB_F32 = 8,
-  NTB_F64 = 9
+  NTB_F64 = 9,
+  NTB_F8E4M3 = 10 /* codes of the paged KV cache only (ntb_kv_*) */
 } NtbDtype;
 
 /* A strided view of device memory.  Strides are in elements and may be 0 (broadcast). */
@@ -302,6 +303,79 @@ NTB_API int ntb_sdpa_decode(const NtbTensor* q, const NtbTensor* k, const NtbTen
 NTB_API int ntb_sdpa_decode_static(const NtbTensor* q, const NtbTensor* k, const NtbTensor* v,
                                    const NtbTensor* mask, const NtbTensor* o, double scale, int causal_variant,
                                    void* stream);
+
+/* ------------------------------------------------------- paged 8-bit KV cache ------------ */
+
+/* A KV cache in pages of T tokens, 8 bits a value with one fp32 scale for each (page, kv head):
+ * value = code * scale.  key, value: codes [P, H, T, D] of one layer, or [L, P, H, T, D] of all
+ * layers where an entry point says so; NTB_F8E4M3 or NTB_I8, any strides with a unit inner one.
+ * key_scale, value_scale: fp32 [P, H] or [L, P, H], any strides.
+ * block_table: int32 [B, M], the page of tokens [m * T, (m + 1) * T) of row b; an entry outside
+ * [0, P) is a hole.  refs: int32 [P], how many times a page is referenced by block tables or by
+ * the caller; 0 = free.  These entry points have no counterpart in the reference. */
+typedef struct {
+  NtbTensor key, value;
+  NtbTensor key_scale, value_scale;
+} NtbKvCache;
+
+/* Quantises key, value [B, H, S, D] (bf16, fp16 or fp32; any strides) into the cache layer: token
+ * i of row b goes to position start[b] + i, for i < counts[b] (counts NULL: S).  Rows with a
+ * negative start, tokens past the table and tokens in holes are dropped.  For each page and head:
+ * s_new = the smallest power of two (between 2^-100 and 2^120) with max |x| <= qmax * s_new over
+ * the page's new finite elements (qmax 448 for e4m3, 127 for int8); where the page holds earlier
+ * tokens of the row the scale becomes max(s_old, s_new) and, if it grows, their codes are
+ * re-rounded; else it becomes s_new.  Codes round to nearest even and saturate; NaN stays NaN in
+ * e4m3 and becomes 0 in int8.  Two rows must not store into the same page. */
+NTB_API int ntb_kv_store(const NtbKvCache* cache, const NtbTensor* key, const NtbTensor* value,
+                         const NtbTensor* block_table, const NtbTensor* start, const NtbTensor* counts,
+                         void* stream);
+
+/* o[b, h, i] = softmax over the keys j < lengths[b] outside holes (and j <= start[b] + i when
+ * causal; start NULL: lengths[b] - Sq) of scale * q . k_j, applied to v_j; zero where no key is
+ * left.  q, o: [B, Hq, Sq, D] of one dtype (bf16, fp16, fp32), any strides with a unit inner one,
+ * Hq a multiple of the cache's heads, D <= 256.  Statistics and sums in fp32.  The cache is read as
+ * one layer.  `workspace` (16-byte aligned device memory of the size the query reports, which
+ * does not depend on the lengths) holds the partial results of key ranges. */
+NTB_API int ntb_kv_attention_workspace(const NtbTensor* q, const NtbKvCache* cache, const NtbTensor* block_table,
+                                       int64_t* bytes);
+NTB_API int ntb_kv_attention(const NtbTensor* q, const NtbKvCache* cache, const NtbTensor* block_table,
+                             const NtbTensor* lengths, const NtbTensor* start, const NtbTensor* o, double scale,
+                             int causal, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Copies pages src[k] -> dst[k] (int32 device lists of one length) with their scales, in every
+ * layer of the [L, P, H, T, D] cache.  No page may be both a source and a destination, nor twice a
+ * destination; pairs with an index outside [0, P) are skipped. */
+NTB_API int ntb_kv_copy_pages(const NtbKvCache* cache, const NtbTensor* src, const NtbTensor* dst, void* stream);
+
+/* Gives every table entry that lengths[b] tokens need and that holds no page the lowest-numbered
+ * free page, in row order.  table_out [B, M], refs_out [P] and missing [1] (how many entries found
+ * no free page; they stay holes) are contiguous and distinct from the inputs; invalid entries of
+ * the table come out as -1.  workspace: 4 * B * M bytes of device memory. */
+NTB_API int ntb_kv_extend(const NtbTensor* block_table, const NtbTensor* lengths, const NtbTensor* refs,
+                          int64_t page_size, const NtbTensor* table_out, const NtbTensor* refs_out,
+                          const NtbTensor* missing, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Makes new row i of the block table continue old row parents[i] (int32 [N]; an index outside
+ * [0, B) makes an empty row): forks rows named several times, frees rows that are not named,
+ * permutes the others.  Full pages are shared.  The first new row that continues an old one keeps
+ * its partly filled last page and any reserved ones; each further one gets a copy of the partly
+ * filled page, in every layer of the [L, P, H, T, D] cache, in the lowest-numbered page that is
+ * free after the old rows' references are gone.  table_out [N, M], lengths_out [N], refs_out [P]
+ * and missing [1] (copies that found no free page; their entries are holes) are contiguous and
+ * distinct from the inputs.  workspace: 4 * (4 * N + 1) bytes of device memory. */
+NTB_API int ntb_kv_reorder(const NtbKvCache* cache, const NtbTensor* block_table, const NtbTensor* lengths,
+                           const NtbTensor* refs, const NtbTensor* parents, const NtbTensor* table_out,
+                           const NtbTensor* lengths_out, const NtbTensor* refs_out, const NtbTensor* missing,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Moves the used pages (refs > 0; there are U = used[0] of them) to the front of the pool: the k-th
+ * used page past the first U moves to the k-th free page among them, in every layer of the
+ * [L, P, H, T, D] cache.  table_out (block_table's shape; entries of free pages come out as -1),
+ * refs_out [P] and used [1] are contiguous and distinct from the inputs.  workspace:
+ * 4 * (3 * P + 1) bytes of device memory. */
+NTB_API int ntb_kv_compact(const NtbKvCache* cache, const NtbTensor* block_table, const NtbTensor* refs,
+                           const NtbTensor* table_out, const NtbTensor* refs_out, const NtbTensor* used,
+                           void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

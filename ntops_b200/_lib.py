@@ -68,6 +68,13 @@ EXPORTS = (
     "ntb_sdpa_decode_workspace",
     "ntb_sdpa_decode",
     "ntb_sdpa_decode_static",
+    "ntb_kv_store",
+    "ntb_kv_attention_workspace",
+    "ntb_kv_attention",
+    "ntb_kv_copy_pages",
+    "ntb_kv_extend",
+    "ntb_kv_reorder",
+    "ntb_kv_compact",
 )
 
 
@@ -81,7 +88,17 @@ class NtbTensor(ctypes.Structure):
     ]
 
 
+class NtbKvCache(ctypes.Structure):
+    _fields_ = [
+        ("key", NtbTensor),
+        ("value", NtbTensor),
+        ("key_scale", NtbTensor),
+        ("value_scale", NtbTensor),
+    ]
+
+
 _P = ctypes.POINTER(NtbTensor)
+_PC = ctypes.POINTER(NtbKvCache)
 _VP = ctypes.c_void_p
 _SIGNATURES = {
     "ntb_version": ([], ctypes.c_int),
@@ -117,6 +134,16 @@ _SIGNATURES = {
         ctypes.c_int,
     ),
     "ntb_sdpa_decode_static": ([_P, _P, _P, _P, _P, ctypes.c_double, ctypes.c_int, _VP], ctypes.c_int),
+    "ntb_kv_store": ([_PC, _P, _P, _P, _P, _P, _VP], ctypes.c_int),
+    "ntb_kv_attention_workspace": ([_P, _PC, _P, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
+    "ntb_kv_attention": (
+        [_P, _PC, _P, _P, _P, _P, ctypes.c_double, ctypes.c_int, _VP, ctypes.c_int64, _VP],
+        ctypes.c_int,
+    ),
+    "ntb_kv_copy_pages": ([_PC, _P, _P, _VP], ctypes.c_int),
+    "ntb_kv_extend": ([_P, _P, _P, ctypes.c_int64, _P, _P, _P, _VP, ctypes.c_int64, _VP], ctypes.c_int),
+    "ntb_kv_reorder": ([_PC, _P, _P, _P, _P, _P, _P, _P, _P, _VP, ctypes.c_int64, _VP], ctypes.c_int),
+    "ntb_kv_compact": ([_PC, _P, _P, _P, _P, _P, _VP, ctypes.c_int64, _VP], ctypes.c_int),
 }
 
 _lib = None

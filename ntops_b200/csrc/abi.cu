@@ -52,6 +52,7 @@ const char* dtype_name(int dt) {
     case NTB_BF16: return "bfloat16";
     case NTB_F32: return "float32";
     case NTB_F64: return "float64";
+    case NTB_F8E4M3: return "float8_e4m3";
     default: return "unknown";
   }
 }

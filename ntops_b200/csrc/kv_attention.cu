@@ -1,0 +1,344 @@
+// ntb_kv_attention: attention of new queries over a paged 8-bit KV cache.
+//
+//   out[b, h, i] = sum_j p_j vs_j vcode_j / sum_j p_j,   p_j = exp(scale * ks_j * (q . kcode_j)),
+// over the keys j < lengths[b] that are not in a hole of the block table and, when causal, not
+// past the query's position start[b] + i; zero where no key is left.  ks_j and vs_j are the
+// scales of token j's page, which multiply scores and probabilities instead of 2 * D values.
+//
+// kv_attention_decode.cu holds the tensor-core kernel for few rows.  This file has the entry
+// points, the kernel for every other case (fp32 queries, any head_dim up to 256, any page size:
+// CUDA-core dot products over 32-key tiles staged in fp32) and the kernel that joins the partial
+// results of segments cut over the key range.
+#include <algorithm>
+
+#include "kv_attention.cuh"
+
+namespace ntb {
+namespace kv {
+namespace {
+
+constexpr int kGenThreads = 128;
+constexpr int kGenTile = 16;   // rows of a tile, four a warp
+constexpr int kGenKeys = 32;   // keys staged at a time
+constexpr int kGenUnit = 128;
+
+// DC: output columns of a lane (head_dim <= 32 * DC).
+template <typename T, int CODE, int DC>
+__global__ void __launch_bounds__(kGenThreads) generic_kernel(AttnArgs a) {
+  extern __shared__ __align__(16) float sm[];
+  const int D = a.c.D;
+  int* pre = reinterpret_cast<int*>(sm);               // [nb + 1]
+  float* Qs = sm + (a.nb + 1);                         // [kGenTile][D]
+  float* Ks = Qs + kGenTile * D;                       // [kGenKeys][D + 1]
+  float* Vs = Ks + kGenKeys * (D + 1);                 // [kGenKeys][D]
+  float* Ps = Vs + kGenKeys * D;                       // [4][kGenKeys]
+  __shared__ int ids[kGenKeys];
+  __shared__ float ksc[kGenKeys], vsc[kGenKeys];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  prefix_units<kGenThreads>(a, pre);
+  const Line line(a, pre);
+  if ((int)blockIdx.x >= line.blocks) return;
+  const int64_t lo = line.begin(blockIdx.x), hi = line.begin(blockIdx.x + 1);
+  for (int64_t pos = lo; pos < hi;) {
+    const Piece pc = piece_at(a, line, pre, pos, lo, hi);
+    pos = pc.next;
+    const int len = row_length(a, pc.b), start = row_start(a, pc.b, len);
+    const int r0 = pc.tile * kGenTile;
+    __syncthreads();  // the previous piece's readers of Qs are done
+    for (int i = threadIdx.x; i < kGenTile * D; i += kGenThreads) {
+      const int r = r0 + i / D, d = i % D;
+      float x = 0.f;
+      if (r < a.rows)
+        x = cvt<float>(reinterpret_cast<const T*>(a.q)[(int64_t)pc.b * a.q_b +
+                                                       (int64_t)(pc.head * a.group + r % a.group) * a.q_h +
+                                                       (int64_t)(r / a.group) * a.q_s + d]);
+      Qs[i] = x;
+    }
+    float m[4], l[4], acc[4][DC];
+    int kmax[4], top = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + warp + 4 * i;
+      kmax[i] = r < a.rows ? last_key(a, len, start, r / a.group) : -1;
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < DC; ++c) acc[i][c] = 0.f;
+    }
+    // the last key that any row of the tile sees ends the loop
+    top = last_key(a, len, start, (min(r0 + kGenTile, a.rows) - 1) / a.group);
+    const int k_end = min(min(len, pc.u1 * kGenUnit), top + 1);
+    for (int k0 = pc.u0 * kGenUnit; k0 < k_end; k0 += kGenKeys) {
+      __syncthreads();
+      if (threadIdx.x < kGenKeys) {
+        const int key = k0 + threadIdx.x;
+        const int id = key < k_end ? page_of(a.table, a.c.P, pc.b, key / a.c.T) : -1;
+        ids[threadIdx.x] = id;
+        ksc[threadIdx.x] = id < 0 ? 0.f : a.c.key_scale[(int64_t)id * a.c.ks_p + (int64_t)pc.head * a.c.ks_h];
+        vsc[threadIdx.x] = id < 0 ? 0.f : a.c.value_scale[(int64_t)id * a.c.vs_p + (int64_t)pc.head * a.c.vs_h];
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < kGenKeys * D; i += kGenThreads) {
+        const int kk = i / D, d = i - kk * D, id = ids[kk];
+        float kv = 0.f, vv = 0.f;
+        if (id >= 0) {
+          const int64_t t = (k0 + kk) % a.c.T;
+          kv = decode1<CODE>(a.c.key[(int64_t)id * a.c.k_p + (int64_t)pc.head * a.c.k_h + t * a.c.k_t + d]) * ksc[kk];
+          vv = decode1<CODE>(a.c.value[(int64_t)id * a.c.v_p + (int64_t)pc.head * a.c.v_h + t * a.c.v_t + d]) * vsc[kk];
+        }
+        Ks[kk * (D + 1) + d] = kv;
+        Vs[kk * D + d] = vv;
+      }
+      __syncthreads();
+      const int key = k0 + lane;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = warp + 4 * i;
+        if (r0 + r >= a.rows) break;
+        float s = -INFINITY;
+        if (key < k_end && key <= kmax[i] && ids[lane] >= 0) {
+          float dot = 0.f;
+          for (int d = 0; d < D; ++d) dot = fmaf(Qs[r * D + d], Ks[lane * (D + 1) + d], dot);
+          s = dot * a.scale * kLog2eF;
+        }
+        float mt = s;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+        const float m_new = fmaxf(m[i], mt);
+        const float m_ref = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2f(m[i] - m_ref), p = exp2f(s - m_ref);
+        float ps = p;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
+        l[i] = l[i] * alpha + ps;
+        m[i] = m_new;
+        Ps[warp * kGenKeys + lane] = p;
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          const int d = lane + 32 * c;
+          if (d < D) {
+            float x = acc[i][c] * alpha;
+            for (int kk = 0; kk < kGenKeys; ++kk) x = fmaf(Ps[warp * kGenKeys + kk], Vs[kk * D + d], x);
+            acc[i][c] = x;
+          }
+        }
+        __syncwarp();
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rt = warp + 4 * i, r = r0 + rt;
+      if (r >= a.rows) break;
+      if (pc.whole) {
+        T* o = reinterpret_cast<T*>(a.o) + (int64_t)pc.b * a.o_b + (int64_t)(pc.head * a.group + r % a.group) * a.o_h +
+               (int64_t)(r / a.group) * a.o_s;
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+#pragma unroll
+        for (int c = 0; c < DC; ++c)
+          if (lane + 32 * c < D) o[lane + 32 * c] = cvt<T>(l[i] == 0.f ? 0.f : acc[i][c] * inv);
+      } else {
+        float* w = a.part + (int64_t)pc.slot * slot_floats(a.tile, D) + (int64_t)rt * (D + 2);
+#pragma unroll
+        for (int c = 0; c < DC; ++c)
+          if (lane + 32 * c < D) w[lane + 32 * c] = acc[i][c];
+        if (lane == 0) {
+          w[D] = m[i];
+          w[D + 1] = l[i];
+        }
+      }
+    }
+  }
+}
+
+// Joins the pieces of every cut segment, one block a segment:
+//   M = max_c m_c,  out = sum_c O_c 2^(m_c - M) / sum_c l_c 2^(m_c - M).
+template <typename T>
+__global__ void __launch_bounds__(128) combine_kernel(AttnArgs a) {
+  extern __shared__ int pre[];
+  prefix_units<128>(a, pre);  // lengths are inputs of the whole call, not of the previous kernel
+  const Line line(a, pre);
+  const int x = blockIdx.x / line.segs, seg = blockIdx.x % line.segs;
+  const int units = pre[x + 1] - pre[x];
+  const int64_t u0 = (int64_t)pre[x] * line.segs + (int64_t)seg * units;
+  const int c0 = line.owner(u0), c1 = line.owner(u0 + units - 1);
+  grid_dependency_wait();
+  if (c0 == c1) return;  // whole: its block wrote the output
+  const int D = a.c.D, b = a.b0 + x, tile = seg / a.c.H, head = seg % a.c.H;
+  for (int rt = 0; rt < a.tile; ++rt) {
+    const int r = tile * a.tile + rt;
+    if (r >= a.rows) break;
+    const float* first = a.part + (int64_t)(2 * c0 + (line.begin(c0) < u0 ? 1 : 0)) * slot_floats(a.tile, D) +
+                         (int64_t)rt * (D + 2);
+    const float* rest = a.part + (int64_t)rt * (D + 2);
+    auto piece = [&](int c) { return c == c0 ? first : rest + (int64_t)2 * c * slot_floats(a.tile, D); };
+    float M = -INFINITY;
+    for (int c = c0; c <= c1; ++c) M = fmaxf(M, piece(c)[D]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    T* o = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_b + (int64_t)(head * a.group + r % a.group) * a.o_h +
+           (int64_t)(r / a.group) * a.o_s;
+    for (int d = threadIdx.x; d < D; d += 128) {
+      float L = 0.f, acc = 0.f;
+      for (int c = c0; c <= c1; ++c) {
+        const float* w = piece(c);
+        const float f = exp2f(w[D] - ref);
+        L = fmaf(w[D + 1], f, L);
+        acc = fmaf(w[d], f, acc);
+      }
+      o[d] = cvt<T>(L == 0.f ? 0.f : acc / L);
+    }
+  }
+}
+
+size_t generic_smem(const AttnArgs& a) {
+  return sizeof(float) * ((size_t)(a.nb + 1) + (size_t)kGenTile * a.c.D + (size_t)kGenKeys * (2 * a.c.D + 1) +
+                          4 * kGenKeys);
+}
+
+template <typename T, int CODE, int DC>
+int generic_go(AttnArgs a, cudaStream_t st, int* blocks) {
+  auto k = generic_kernel<T, CODE, DC>;
+  const size_t smem = generic_smem(a);
+  NTB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+  if (blocks != nullptr) {
+    *blocks = resident_blocks((const void*)k, kGenThreads, smem);
+    return NTB_OK;
+  }
+  k<<<a.G, kGenThreads, smem, st>>>(a);
+  NTB_LAUNCH_CHECK();
+  return NTB_OK;
+}
+
+template <typename T>
+int generic_typed(const AttnArgs& a, cudaStream_t st, int* blocks) {
+  const bool wide = a.c.D > 128;
+  if (a.c.code == NTB_F8E4M3)
+    return wide ? generic_go<T, NTB_F8E4M3, 8>(a, st, blocks) : generic_go<T, NTB_F8E4M3, 4>(a, st, blocks);
+  return wide ? generic_go<T, NTB_I8, 8>(a, st, blocks) : generic_go<T, NTB_I8, 4>(a, st, blocks);
+}
+
+// Launches the generic kernel, or with `blocks` only asks how many of its blocks are resident.
+int generic_any(const AttnArgs& a, int dtype, cudaStream_t st, int* blocks) {
+  switch (dtype) {
+    case NTB_BF16: return generic_typed<__nv_bfloat16>(a, st, blocks);
+    case NTB_F16: return generic_typed<__half>(a, st, blocks);
+    default: return generic_typed<float>(a, st, blocks);
+  }
+}
+
+int combine_launch(const AttnArgs& a, int dtype, cudaStream_t st) {
+  // One unit for every segment at most: nothing can be cut.
+  if ((int64_t)a.table.M * a.c.T <= a.unit) return NTB_OK;
+  const int64_t grid = (int64_t)a.nb * a.tiles * a.c.H;
+  const size_t smem = sizeof(int) * (a.nb + 1);
+  auto go = [&](auto k) -> int {
+    NTB_CUDA(launch_dependent(k, dim3((unsigned)grid), dim3(128), smem, st, a));
+    return NTB_OK;
+  };
+  switch (dtype) {
+    case NTB_BF16: return go(combine_kernel<__nv_bfloat16>);
+    case NTB_F16: return go(combine_kernel<__half>);
+    default: return go(combine_kernel<float>);
+  }
+}
+
+// Checks the shared arguments and fills everything but the kernel's own plan.
+int fill(const NtbTensor* q, const NtbKvCache* cache, const NtbTensor* table, AttnArgs* a) {
+  int rc;
+  if ((rc = check_tensor(q, "query")) != NTB_OK) return rc;
+  if ((rc = check_cache(cache, false, &a->c)) != NTB_OK) return rc;
+  if ((rc = check_i32(table, 2, "block_table")) != NTB_OK) return rc;
+  NTB_ARG(q->ndim == 4, "query must be 4-D [B, Hq, Sq, D]");
+  NTB_UNSUP(q->dtype == NTB_BF16 || q->dtype == NTB_F16 || q->dtype == NTB_F32,
+            "query must be bfloat16, float16 or float32, got %s", dtype_name(q->dtype));
+  NTB_ARG(q->stride[3] == 1 || q->shape[3] == 1, "query must have a unit inner stride");
+  NTB_ARG(q->shape[3] == a->c.D, "query head_dim %lld differs from the cache's %d", (long long)q->shape[3], a->c.D);
+  NTB_ARG(q->shape[1] > 0 && q->shape[1] % a->c.H == 0, "query heads must be a multiple of the cache's heads");
+  NTB_ARG(table->shape[0] == q->shape[0], "block_table rows differ from the batch");
+  NTB_UNSUP(a->c.D <= 256, "head_dim above 256 is not supported");
+  NTB_ARG(q->shape[0] <= 0x7fffffffLL && q->shape[2] <= 0x7fffffffLL && q->shape[1] <= 65535 &&
+              q->shape[1] / a->c.H * q->shape[2] <= 0x7fffffffLL && table->shape[1] <= 0x7fffffffLL &&
+              table->shape[1] * a->c.T <= 0x7fffffffLL,
+          "kv_attention: a dimension is too large");
+  a->q = q->data;
+  a->q_b = q->stride[0]; a->q_h = q->stride[1]; a->q_s = q->stride[2];
+  a->Hq = (int)q->shape[1];
+  a->Sq = (int)q->shape[2];
+  a->group = a->Hq / a->c.H;
+  a->rows = a->group * a->Sq;
+  a->table = {reinterpret_cast<const int*>(table->data), table->stride[0], table->stride[1], (int)q->shape[0],
+              (int)table->shape[1]};
+  a->err = device_error_ptr();
+  return NTB_OK;
+}
+
+// Tile, unit and number of blocks for a launch of up to kMaxBatch batch rows.
+int plan(AttnArgs* a, int dtype) {
+  a->b0 = 0;
+  a->nb = std::min(a->table.B, kMaxBatch);
+  a->tile = kGenTile;
+  a->unit = kGenUnit;
+  a->tiles = (a->rows + a->tile - 1) / a->tile;
+  return generic_any(*a, dtype, nullptr, &a->G);
+}
+
+int64_t part_bytes(const AttnArgs& a) { return 2ll * a.G * slot_floats(a.tile, a.c.D) * (int64_t)sizeof(float); }
+
+}  // namespace
+}  // namespace kv
+}  // namespace ntb
+
+extern "C" int ntb_kv_attention_workspace(const NtbTensor* q, const NtbKvCache* cache, const NtbTensor* block_table,
+                                          int64_t* bytes) {
+  using namespace ntb;
+  using namespace ntb::kv;
+  NTB_ARG(bytes != nullptr, "bytes is NULL");
+  AttnArgs a = {};
+  int rc = fill(q, cache, block_table, &a);
+  if (rc != NTB_OK) return rc;
+  *bytes = 0;
+  if ((int64_t)a.table.B * a.rows == 0) return NTB_OK;
+  if ((rc = plan(&a, q->dtype)) != NTB_OK) return rc;
+  *bytes = part_bytes(a);
+  return NTB_OK;
+}
+
+extern "C" int ntb_kv_attention(const NtbTensor* q, const NtbKvCache* cache, const NtbTensor* block_table,
+                                const NtbTensor* lengths, const NtbTensor* start, const NtbTensor* o, double scale,
+                                int causal, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace ntb;
+  using namespace ntb::kv;
+  AttnArgs a = {};
+  int rc = fill(q, cache, block_table, &a);
+  if (rc != NTB_OK) return rc;
+  if ((rc = check_i32(lengths, 1, "lengths")) != NTB_OK) return rc;
+  if (start != nullptr && (rc = check_i32(start, 1, "start")) != NTB_OK) return rc;
+  if ((rc = check_tensor(o, "output")) != NTB_OK) return rc;
+  NTB_ARG(lengths->shape[0] == q->shape[0], "lengths differs from the batch");
+  NTB_ARG(start == nullptr || start->shape[0] == q->shape[0], "start differs from the batch");
+  NTB_ARG(same_shape(o, q), "output must be shaped like the query");
+  NTB_ARG(o->stride[3] == 1 || o->shape[3] == 1, "output must have a unit inner stride");
+  NTB_UNSUP(o->dtype == q->dtype, "output dtype must equal the query dtype");
+  if ((int64_t)a.table.B * a.rows == 0) return NTB_OK;
+  a.o = o->data;
+  a.o_b = o->stride[0]; a.o_h = o->stride[1]; a.o_s = o->stride[2];
+  a.lengths = reinterpret_cast<const int*>(lengths->data);
+  a.len_s = lengths->stride[0];
+  a.start = start ? reinterpret_cast<const int*>(start->data) : nullptr;
+  a.st_s = start ? start->stride[0] : 0;
+  a.scale = (float)scale;
+  a.causal = causal != 0;
+  if ((rc = plan(&a, q->dtype)) != NTB_OK) return rc;
+  NTB_ARG(workspace != nullptr && workspace_bytes >= part_bytes(a), "workspace too small: %lld bytes, need %lld",
+          (long long)workspace_bytes, (long long)part_bytes(a));
+  NTB_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
+  a.part = reinterpret_cast<float*>(workspace);
+  cudaStream_t st = (cudaStream_t)stream;
+  NTB_UNSUP((int64_t)kMaxBatch * a.tiles * a.c.H <= 0x7fffffffLL, "kv_attention: too many query rows");
+  for (a.b0 = 0; a.b0 < a.table.B; a.b0 += kMaxBatch) {
+    a.nb = std::min(a.table.B - a.b0, kMaxBatch);
+    if ((rc = generic_any(a, q->dtype, st, nullptr)) != NTB_OK) return rc;
+    if ((rc = combine_launch(a, q->dtype, st)) != NTB_OK) return rc;
+  }
+  return NTB_OK;
+}

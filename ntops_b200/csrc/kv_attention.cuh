@@ -1,0 +1,146 @@
+// Attention over the paged 8-bit KV cache: arguments, the split of the work over the key range,
+// and the partial results that it leaves (kv_attention.cu, kv_attention_decode.cu,
+// kv_attention_sm100.cu).
+//
+// The rows of one (batch row, kv head) are packed: row r = s * group + g is query s of the
+// group's query head g, so a tile of rows covers few query positions and reads each key once for
+// the whole group.  A segment is a (batch row, row tile, kv head); its keys are cut into units of
+// `unit` keys, at least one.  The units of all segments, in the order batch row, tile, head,
+// key, form one line that the resident blocks divide evenly, whatever the lengths are: lengths
+// live on the device, so every block derives its share itself.  A segment that one block holds
+// whole is written out by it; a cut one leaves partial results (max, sum and unnormalised O for
+// each row) that combine_kernel joins.  A block cuts at most the first and the last segment of
+// its share, hence two slots for each block.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace ntb {
+namespace kv {
+
+constexpr float kLog2eF = 1.4426950408889634f;
+constexpr int kMaxBatch = 4096;  // batch rows of one launch (their unit counts sit in shared memory)
+
+struct AttnArgs {
+  const void* q;
+  void* o;
+  Layer c;
+  Table table;
+  const int *lengths, *start;  // start null: length - Sq
+  int64_t len_s, st_s;
+  int64_t q_b, q_h, q_s, o_b, o_h, o_s;
+  int Hq, Sq, group, causal;
+  float scale;
+  int b0, nb;        // batch rows of this launch
+  int rows;          // group * Sq
+  int tile, tiles;   // rows of a tile, tiles of a segment row
+  int unit;          // keys of a unit
+  int G;             // blocks that share the work
+  float* part;       // [2 * G][tile][D + 2]: O, then max (base 2), sum
+  unsigned int* err; // device error word (bounded waits)
+};
+
+__host__ __device__ inline int64_t slot_floats(int tile, int D) { return (int64_t)tile * (D + 2); }
+
+// Tokens that row b of the table can hold, and its length within that.
+__device__ __forceinline__ int row_length(const AttnArgs& a, int b) {
+  const int64_t cap = (int64_t)a.table.M * a.c.T;
+  const int len = a.lengths[(int64_t)b * a.len_s];
+  return len < 0 ? 0 : (int)min((int64_t)len, cap);
+}
+__device__ __forceinline__ int row_start(const AttnArgs& a, int b, int len) {
+  return a.start == nullptr ? len - a.Sq : a.start[(int64_t)b * a.st_s];
+}
+__device__ __forceinline__ int row_units(const AttnArgs& a, int b) {
+  return max(1, (row_length(a, b) + a.unit - 1) / a.unit);
+}
+
+// pre[i] = units of the launch's first i batch rows (pre has nb + 1 entries); all threads call it.
+template <int THREADS>
+__device__ __forceinline__ void prefix_units(const AttnArgs& a, int* pre) {
+  __shared__ int part[THREADS / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  for (int i0 = 0; i0 < a.nb; i0 += THREADS) {
+    const int i = i0 + threadIdx.x;
+    int x = i < a.nb ? row_units(a, a.b0 + i) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) part[warp] = x;
+    __syncthreads();
+    int before = base, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += part[w];
+      total += part[w];
+    }
+    if (i < a.nb) pre[i + 1] = before + x;
+    base += total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) pre[0] = 0;
+  __syncthreads();
+}
+
+// The line of units and its division among the blocks.
+struct Line {
+  int64_t total;
+  int segs, blocks;
+  __device__ __forceinline__ Line(const AttnArgs& a, const int* pre) {
+    segs = a.tiles * a.c.H;
+    total = (int64_t)pre[a.nb] * segs;
+    blocks = (int)min((int64_t)a.G, total);
+  }
+  __device__ __forceinline__ int64_t begin(int i) const { return total * i / blocks; }
+  // the block whose share holds unit u
+  __device__ __forceinline__ int owner(int64_t u) const { return (int)(((u + 1) * blocks - 1) / total); }
+};
+
+// One segment's piece of a block's share.
+struct Piece {
+  int b, tile, head;  // batch row, row tile, kv head
+  int u0, u1;         // units [u0, u1) of the segment
+  bool whole;
+  int slot;           // of the partial results where not whole
+  int64_t next;       // position after it
+};
+__device__ __forceinline__ Piece piece_at(const AttnArgs& a, const Line& line, const int* pre, int64_t pos, int64_t lo,
+                                          int64_t hi) {
+  int x = 0, y = a.nb - 1;  // last row whose units begin at or before pos
+  while (x < y) {
+    const int m = (x + y + 1) >> 1;
+    if ((int64_t)pre[m] * line.segs <= pos) x = m;
+    else y = m - 1;
+  }
+  const int units = pre[x + 1] - pre[x];
+  const int64_t rem = pos - (int64_t)pre[x] * line.segs;
+  const int seg = (int)(rem / units);
+  Piece p;
+  p.b = a.b0 + x;
+  p.tile = seg / a.c.H;
+  p.head = seg % a.c.H;
+  p.u0 = (int)(rem - (int64_t)seg * units);
+  p.u1 = (int)min((int64_t)units, p.u0 + (hi - pos));
+  p.whole = p.u0 == 0 && p.u1 == units;
+  p.slot = 2 * (int)blockIdx.x + (pos == lo ? 0 : 1);
+  p.next = pos + (p.u1 - p.u0);
+  return p;
+}
+
+// Last key that query s of a row may see (-1: none).
+__device__ __forceinline__ int last_key(const AttnArgs& a, int len, int start, int s) {
+  if (!a.causal) return len - 1;
+  const int64_t p = (int64_t)start + s;
+  return p < 0 ? -1 : (int)min(p, (int64_t)len - 1);
+}
+
+// Launchers of the kernels; they fill tile / unit / G, and take `part` from the workspace.
+bool decode_takes(const AttnArgs& a, int dtype);
+int decode_plan(AttnArgs* a, int dtype);
+int decode_launch(const AttnArgs& a, int dtype, cudaStream_t st);
+
+}  // namespace kv
+}  // namespace ntb

@@ -1,0 +1,539 @@
+// Page operations of the paged 8-bit KV cache: ntb_kv_copy_pages, ntb_kv_extend, ntb_kv_reorder,
+// ntb_kv_compact.  All run on the device without a host round trip, so they can sit inside a
+// captured step: which pages are free, copied or moved is decided by the kernels from refs
+// (int32 [P]: how many times each page is referenced; 0 = free).
+//
+// Everything that hands out pages takes the lowest-numbered free ones in a fixed order of
+// requests, found with prefix sums, so results do not depend on the order threads run in (the
+// only atomics are integer additions).  A copied page's source is always a page that stays in
+// use and its destination one that nobody references, so copies never overlap.
+#include <algorithm>
+
+#include "kv_cache.cuh"
+#include "rowstage.cuh"
+
+namespace ntb {
+namespace kv {
+namespace {
+
+// ------------------------------------------------------------------------------- copy -----
+// A page of one layer is H * T * D bytes in any order of those dimensions.  Where they are dense
+// a page is one block of bytes and copies as 16-byte vectors; source and destination share the
+// strides, so their order does not matter.
+struct CopyArgs {
+  uint8_t* code[2];     // key, value
+  float* scale[2];
+  int64_t c_l[2], c_p[2], c_h[2], c_t[2], s_l[2], s_p[2], s_h[2];
+  int L, P, H, T, D;
+  int64_t block;        // H * T * D
+  int dense;            // 16-byte vectors over the block
+  const int *src, *dst; // pair lists on the device
+  int64_t src_s, dst_s; // their strides
+  const int* count;     // number of pairs; null: `pairs`
+  int pairs;            // capacity of the lists
+};
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 4;
+constexpr int kCopyChunk = kCopyThreads * kCopyUnroll * 16;  // bytes of a work item
+
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(CopyArgs a) {
+  grid_dependency_wait();
+  const int pairs = a.count == nullptr ? a.pairs : min(max(*a.count, 0), a.pairs);
+  const int chunks = (int)((a.block + kCopyChunk - 1) / kCopyChunk);
+  const int64_t items = (int64_t)pairs * a.L * 2 * chunks;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    int64_t r = it;
+    const int c = (int)(r % chunks);
+    r /= chunks;
+    const int w = (int)(r & 1);
+    r >>= 1;
+    const int l = (int)(r % a.L);
+    const int64_t k = r / a.L;
+    const int src = a.src[k * a.src_s], dst = a.dst[k * a.dst_s];
+    if ((unsigned)src >= (unsigned)a.P || (unsigned)dst >= (unsigned)a.P || src == dst) continue;
+    const uint8_t* s = a.code[w] + (int64_t)l * a.c_l[w] + (int64_t)src * a.c_p[w];
+    uint8_t* d = a.code[w] + (int64_t)l * a.c_l[w] + (int64_t)dst * a.c_p[w];
+    const int64_t lo = (int64_t)c * kCopyChunk, hi = min(a.block, lo + kCopyChunk);
+    if (a.dense) {
+      uint4 v[kCopyUnroll];
+#pragma unroll
+      for (int u = 0; u < kCopyUnroll; ++u) {
+        const int64_t o = lo + ((int64_t)u * kCopyThreads + threadIdx.x) * 16;
+        if (o < hi) v[u] = __ldcs(reinterpret_cast<const uint4*>(s + o));
+      }
+#pragma unroll
+      for (int u = 0; u < kCopyUnroll; ++u) {
+        const int64_t o = lo + ((int64_t)u * kCopyThreads + threadIdx.x) * 16;
+        if (o < hi) __stcs(reinterpret_cast<uint4*>(d + o), v[u]);
+      }
+    } else {
+      for (int64_t o = lo + threadIdx.x; o < hi; o += kCopyThreads) {
+        const int64_t h = o / ((int64_t)a.T * a.D), q = o % ((int64_t)a.T * a.D);
+        const int64_t at = h * a.c_h[w] + (q / a.D) * a.c_t[w] + q % a.D;
+        d[at] = s[at];
+      }
+    }
+    if (c == 0)
+      for (int h = threadIdx.x; h < a.H; h += kCopyThreads) {
+        float* sc = a.scale[w] + (int64_t)l * a.s_l[w] + (int64_t)h * a.s_h[w];
+        sc[(int64_t)dst * a.s_p[w]] = sc[(int64_t)src * a.s_p[w]];
+      }
+  }
+}
+
+int fill_copy(const NtbKvCache* c, CopyArgs* a) {
+  Layer l;
+  int rc = check_cache(c, true, &l);
+  if (rc != NTB_OK) return rc;
+  const NtbTensor* code[2] = {&c->key, &c->value};
+  const NtbTensor* scale[2] = {&c->key_scale, &c->value_scale};
+  a->L = (int)c->key.shape[0];
+  a->P = l.P; a->H = l.H; a->T = l.T; a->D = l.D;
+  a->block = (int64_t)l.H * l.T * l.D;
+  a->dense = a->block % 16 == 0;
+  for (int i = 0; i < 2; ++i) {
+    a->code[i] = reinterpret_cast<uint8_t*>(code[i]->data);
+    a->scale[i] = reinterpret_cast<float*>(scale[i]->data);
+    a->c_l[i] = code[i]->stride[0]; a->c_p[i] = code[i]->stride[1];
+    a->c_h[i] = code[i]->stride[2]; a->c_t[i] = code[i]->stride[3];
+    a->s_l[i] = scale[i]->stride[0]; a->s_p[i] = scale[i]->stride[1]; a->s_h[i] = scale[i]->stride[2];
+    // dense in either order of heads and tokens (size-1 dimensions do not matter)
+    auto is = [](int64_t n, int64_t stride, int64_t want) { return n == 1 || stride == want; };
+    const bool ht = is(l.T, a->c_t[i], l.D) && is(l.H, a->c_h[i], (int64_t)l.T * l.D);
+    const bool th = is(l.H, a->c_h[i], l.D) && is(l.T, a->c_t[i], (int64_t)l.H * l.D);
+    if (!(ht || th) || reinterpret_cast<uintptr_t>(a->code[i]) % 16 != 0 || (a->L > 1 && a->c_l[i] % 16 != 0) ||
+        (a->P > 1 && a->c_p[i] % 16 != 0))
+      a->dense = 0;
+  }
+  return NTB_OK;
+}
+
+int launch_copy(const CopyArgs& a, cudaStream_t st) {
+  const int64_t chunks = (a.block + kCopyChunk - 1) / kCopyChunk;
+  const int64_t most = (int64_t)a.pairs * a.L * 2 * chunks;
+  if (most == 0) return NTB_OK;
+  const int64_t grid = std::min<int64_t>(most, resident_blocks((const void*)copy_kernel, kCopyThreads, 0));
+  NTB_CUDA(launch_dependent(copy_kernel, dim3((unsigned)grid), dim3(kCopyThreads), 0, st, a));
+  return NTB_OK;
+}
+
+// ------------------------------------------------------------------------- allocation -----
+constexpr int kPlanThreads = 1024;
+
+// Exclusive prefix sum of v over the block, and the block's total.
+__device__ __forceinline__ int block_scan(int v, int* total) {
+  __shared__ int part[kPlanThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the previous call's readers are done
+  if (lane == 31) part[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int p = part[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, p, o);
+      if (lane >= o) p += y;
+    }
+    part[lane] = p;
+  }
+  __syncthreads();
+  *total = part[kPlanThreads / 32 - 1];
+  return (warp ? part[warp - 1] : 0) + x - v;
+}
+
+// Gives the lowest free pages (refs 0) to the requests 0 .. wanted - 1 in their order: take(k, p)
+// for request k and page p, whose refs become 1.  Returns how many requests got a page.
+template <typename Take>
+__device__ __forceinline__ int assign_free(int* refs, int P, int wanted, Take take) {
+  constexpr int E = 4;
+  int got = 0;
+  for (int p0 = 0; p0 < P && got < wanted; p0 += kPlanThreads * E) {  // `got` is the same for all threads
+    const int p = p0 + (int)threadIdx.x * E;
+    bool f[E];
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      f[e] = p + e < P && refs[p + e] == 0;
+      n += f[e];
+    }
+    int total;
+    int k = got + block_scan(n, &total);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (f[e]) {
+        if (k < wanted) {
+          refs[p + e] = 1;
+          take(k, p + e);
+        }
+        ++k;
+      }
+    got = min(wanted, got + total);
+  }
+  return got;
+}
+
+struct ExtendArgs {
+  Table in;
+  int* out;            // [B, M] contiguous
+  const int* lengths;
+  int64_t len_s;
+  int* refs;           // a copy of the caller's, updated
+  int P, T;
+  int* missing;
+  int* want;           // [B * M] flat positions without a page
+};
+
+// Copies the table and lists, in row order, the entries that a row's length covers but that hold
+// no page; then hands out pages.  One block: a table is some ten thousand entries.
+__global__ void __launch_bounds__(kPlanThreads) extend_kernel(ExtendArgs a) {
+  const int64_t n = (int64_t)a.in.B * a.in.M;
+  int wanted = 0;
+  for (int64_t i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    int need = 0;
+    if (i < n) {
+      const int b = (int)(i / a.in.M), m = (int)(i % a.in.M);
+      const int id = page_of(a.in, a.P, b, m);
+      need = id < 0 && (int64_t)m * a.T < a.lengths[(int64_t)b * a.len_s];
+      a.out[i] = id;
+    }
+    int total;
+    const int k = wanted + block_scan(need, &total);
+    if (need) a.want[k] = (int)i;
+    wanted += total;
+  }
+  __syncthreads();  // want[] is written
+  const int got = assign_free(a.refs, a.P, wanted, [&](int k, int p) { a.out[a.want[k]] = p; });
+  if (threadIdx.x == 0) *a.missing = wanted - got;
+}
+
+struct ReorderArgs {
+  Table in;
+  int* out;                    // [N, M] contiguous
+  const int *lengths, *parents;
+  int64_t len_s, par_s;
+  int* new_lengths;            // [N]
+  int* refs;                   // a copy of the caller's, updated
+  int N, P, T;
+  int* missing;
+  int *need, *want, *src, *dst, *count;  // workspace: [N] each, and one
+};
+
+// One block a row.  Blocks of old rows take their references away; blocks of new rows write the
+// row, add its references and note the page it needs its own copy of.
+__global__ void __launch_bounds__(128) reorder_rows_kernel(ReorderArgs a) {
+  const int M = a.in.M;
+  if ((int)blockIdx.x < a.in.B) {
+    for (int m = threadIdx.x; m < M; m += blockDim.x) {
+      const int id = page_of(a.in, a.P, blockIdx.x, m);
+      if (id >= 0) atomicSub(&a.refs[id], 1);
+    }
+  }
+  if ((int)blockIdx.x < a.N) {
+    const int i = blockIdx.x;
+    const int p = a.parents[(int64_t)i * a.par_s];
+    const bool ok = (unsigned)p < (unsigned)a.in.B;
+    int earlier = 0;  // does an earlier new row continue the same old row?
+    for (int j = threadIdx.x; j < i; j += blockDim.x) earlier |= a.parents[(int64_t)j * a.par_s] == p;
+    const bool first = !__syncthreads_or(earlier);
+    const int len = ok ? max(a.lengths[(int64_t)p * a.len_s], 0) : 0;
+    const int whole = len / a.T, part = len % a.T;
+    if (threadIdx.x == 0) {
+      a.new_lengths[i] = len;
+      a.need[i] = ok && !first && part ? page_of(a.in, a.P, p, whole) : -1;
+    }
+    for (int m = threadIdx.x; m < M; m += blockDim.x) {
+      const int id = ok && (first || m < whole) ? page_of(a.in, a.P, p, m) : -1;
+      a.out[(int64_t)i * M + m] = id;
+      if (id >= 0) atomicAdd(&a.refs[id], 1);
+    }
+  }
+}
+
+// Hands pages to the new rows that need a copy, in row order, and lists the copies.
+__global__ void __launch_bounds__(kPlanThreads) reorder_assign_kernel(ReorderArgs a) {
+  grid_dependency_wait();
+  int wanted = 0;
+  for (int i0 = 0; i0 < a.N; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    const int need = i < a.N && a.need[i] >= 0;
+    int total;
+    const int k = wanted + block_scan(need, &total);
+    if (need) a.want[k] = i;
+    wanted += total;
+  }
+  __syncthreads();
+  const int got = assign_free(a.refs, a.P, wanted, [&](int k, int p) {
+    const int i = a.want[k];
+    a.src[k] = a.need[i];
+    a.dst[k] = p;
+    a.out[(int64_t)i * a.in.M + a.new_lengths[i] / a.T] = p;
+  });
+  if (threadIdx.x == 0) {
+    *a.count = got;
+    *a.missing = wanted - got;
+  }
+}
+
+struct CompactArgs {
+  Table in;
+  int* out;
+  const int* refs;
+  int64_t ref_s;
+  int* new_refs;               // [P]
+  int* used;
+  int P;
+  int *map, *src, *dst, *count;  // workspace: [P] each, and one
+};
+
+// Counts the used pages U, lists the used pages past the first U and the free pages among them,
+// both in ascending order: the k-th of the one moves to the k-th of the other.
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs a) {
+  int n = 0, U, total;
+  for (int p = threadIdx.x; p < a.P; p += kPlanThreads) n += a.refs[(int64_t)p * a.ref_s] > 0;
+  block_scan(n, &U);
+  int movers = 0, holes = 0;
+  for (int p0 = 0; p0 < a.P; p0 += kPlanThreads) {
+    const int p = p0 + threadIdx.x;
+    const int ref = p < a.P ? a.refs[(int64_t)p * a.ref_s] : 0;
+    const bool u = ref > 0;
+    const int kind = p >= a.P ? 0 : (p >= U ? (u ? 1 : 0) : (u ? 0 : 1 << 16));
+    const int k = block_scan(kind, &total);
+    if (kind == 1) a.src[movers + (k & 0xFFFF)] = p;
+    else if (kind) a.dst[holes + (k >> 16)] = p;
+    movers += total & 0xFFFF;
+    holes += total >> 16;
+    if (p < a.P) {
+      a.map[p] = u ? p : -1;
+      a.new_refs[p] = u && p < U ? ref : 0;
+    }
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < movers; k += kPlanThreads) {
+    a.map[a.src[k]] = a.dst[k];
+    a.new_refs[a.dst[k]] = a.refs[(int64_t)a.src[k] * a.ref_s];
+  }
+  if (threadIdx.x == 0) {
+    *a.count = movers;
+    *a.used = U;
+  }
+}
+
+__global__ void __launch_bounds__(256) compact_table_kernel(CompactArgs a) {
+  grid_dependency_wait();
+  const int64_t n = (int64_t)a.in.B * a.in.M;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int id = page_of(a.in, a.P, (int)(i / a.in.M), (int)(i % a.in.M));
+    a.out[i] = id < 0 ? -1 : a.map[id];
+  }
+}
+
+int fill_table(const NtbTensor* t, const char* name, Table* out) {
+  int rc = check_i32(t, 2, name);
+  if (rc != NTB_OK) return rc;
+  NTB_ARG(t->shape[0] <= 0x7fffffffLL && t->shape[1] <= 0x7fffffffLL && numel(t) <= 0x7fffffffLL, "%s is too large",
+          name);
+  *out = {reinterpret_cast<const int*>(t->data), t->stride[0], t->stride[1], (int)t->shape[0], (int)t->shape[1]};
+  return NTB_OK;
+}
+
+// An int32 output the kernels index densely.
+int check_out(const NtbTensor* t, int ndim, const char* name) {
+  int rc = check_i32(t, ndim, name);
+  if (rc != NTB_OK) return rc;
+  NTB_ARG(is_contiguous(t), "%s must be contiguous", name);
+  return NTB_OK;
+}
+
+// refs_out = refs, on the stream.
+int copy_refs(const NtbTensor* refs, const NtbTensor* out, cudaStream_t st) {
+  if (numel(refs) == 0) return NTB_OK;
+  NTB_CUDA(cudaMemcpyAsync(out->data, refs->data, (size_t)numel(refs) * 4, cudaMemcpyDeviceToDevice, st));
+  return NTB_OK;
+}
+
+}  // namespace
+
+int resident_blocks(const void* kernel, int threads, size_t smem) {
+  return rs::blocks_per_sm_smem(kernel, threads, smem) * sm_count();
+}
+
+}  // namespace kv
+}  // namespace ntb
+
+extern "C" int ntb_kv_copy_pages(const NtbKvCache* cache, const NtbTensor* src, const NtbTensor* dst, void* stream) {
+  using namespace ntb;
+  using namespace ntb::kv;
+  CopyArgs a = {};
+  int rc;
+  if ((rc = fill_copy(cache, &a)) != NTB_OK) return rc;
+  if ((rc = check_i32(src, 1, "src")) != NTB_OK) return rc;
+  if ((rc = check_i32(dst, 1, "dst")) != NTB_OK) return rc;
+  NTB_ARG(src->shape[0] == dst->shape[0], "src and dst lengths differ");
+  NTB_ARG(src->shape[0] <= 0x7fffffffLL, "too many pages");
+  a.src = reinterpret_cast<const int*>(src->data);
+  a.dst = reinterpret_cast<const int*>(dst->data);
+  a.src_s = src->stride[0];
+  a.dst_s = dst->stride[0];
+  a.pairs = (int)src->shape[0];
+  return launch_copy(a, (cudaStream_t)stream);
+}
+
+extern "C" int ntb_kv_extend(const NtbTensor* block_table, const NtbTensor* lengths, const NtbTensor* refs,
+                             int64_t page_size, const NtbTensor* table_out, const NtbTensor* refs_out,
+                             const NtbTensor* missing, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace ntb;
+  using namespace ntb::kv;
+  ExtendArgs a = {};
+  int rc;
+  if ((rc = fill_table(block_table, "block_table", &a.in)) != NTB_OK) return rc;
+  if ((rc = check_i32(lengths, 1, "lengths")) != NTB_OK) return rc;
+  if ((rc = check_out(refs, 1, "refs")) != NTB_OK) return rc;
+  if ((rc = check_out(table_out, 2, "table_out")) != NTB_OK) return rc;
+  if ((rc = check_out(refs_out, 1, "refs_out")) != NTB_OK) return rc;
+  if ((rc = check_out(missing, 1, "missing")) != NTB_OK) return rc;
+  NTB_ARG(page_size > 0 && page_size <= 0x7fffffffLL, "page_size must be positive");
+  NTB_ARG(lengths->shape[0] == block_table->shape[0], "lengths differs from the batch");
+  NTB_ARG(same_shape(table_out, block_table) && same_shape(refs_out, refs) && missing->shape[0] == 1,
+          "outputs must be shaped like block_table, refs and [1]");
+  NTB_ARG(refs->shape[0] <= 0x7fffffffLL, "too many pages");
+  NTB_ARG(refs_out->data != refs->data && (table_out->data != block_table->data || numel(block_table) == 0),
+          "outputs must not be the inputs");
+  const int64_t need = 4 * numel(block_table);
+  NTB_ARG(workspace_bytes >= need && (workspace != nullptr || need == 0), "workspace too small: %lld bytes, need %lld",
+          (long long)workspace_bytes, (long long)need);
+  cudaStream_t st = (cudaStream_t)stream;
+  if ((rc = copy_refs(refs, refs_out, st)) != NTB_OK) return rc;
+  a.out = reinterpret_cast<int*>(table_out->data);
+  a.lengths = reinterpret_cast<const int*>(lengths->data);
+  a.len_s = lengths->stride[0];
+  a.refs = reinterpret_cast<int*>(refs_out->data);
+  a.P = (int)refs->shape[0];
+  a.T = (int)page_size;
+  a.missing = reinterpret_cast<int*>(missing->data);
+  a.want = reinterpret_cast<int*>(workspace);
+  extend_kernel<<<1, kPlanThreads, 0, st>>>(a);
+  NTB_LAUNCH_CHECK();
+  return NTB_OK;
+}
+
+extern "C" int ntb_kv_reorder(const NtbKvCache* cache, const NtbTensor* block_table, const NtbTensor* lengths,
+                              const NtbTensor* refs, const NtbTensor* parents, const NtbTensor* table_out,
+                              const NtbTensor* lengths_out, const NtbTensor* refs_out, const NtbTensor* missing,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace ntb;
+  using namespace ntb::kv;
+  CopyArgs c = {};
+  ReorderArgs a = {};
+  int rc;
+  if ((rc = fill_copy(cache, &c)) != NTB_OK) return rc;
+  if ((rc = fill_table(block_table, "block_table", &a.in)) != NTB_OK) return rc;
+  if ((rc = check_i32(lengths, 1, "lengths")) != NTB_OK) return rc;
+  if ((rc = check_i32(parents, 1, "parents")) != NTB_OK) return rc;
+  if ((rc = check_out(refs, 1, "refs")) != NTB_OK) return rc;
+  if ((rc = check_out(table_out, 2, "table_out")) != NTB_OK) return rc;
+  if ((rc = check_out(lengths_out, 1, "lengths_out")) != NTB_OK) return rc;
+  if ((rc = check_out(refs_out, 1, "refs_out")) != NTB_OK) return rc;
+  if ((rc = check_out(missing, 1, "missing")) != NTB_OK) return rc;
+  const int64_t N = parents->shape[0];
+  NTB_ARG(lengths->shape[0] == block_table->shape[0], "lengths differs from the batch");
+  NTB_ARG(refs->shape[0] == c.P && refs_out->shape[0] == c.P, "refs must have one entry for each page");
+  NTB_ARG(table_out->shape[0] == N && table_out->shape[1] == block_table->shape[1] && lengths_out->shape[0] == N &&
+              missing->shape[0] == 1,
+          "outputs must be shaped [N, M], [N] and [1]");
+  NTB_ARG(N * block_table->shape[1] <= 0x7fffffffLL && N <= 0x7fffffffLL, "too many rows");
+  NTB_ARG(refs_out->data != refs->data || c.P == 0, "outputs must not be the inputs");
+  NTB_ARG((table_out->data != block_table->data || numel(table_out) == 0) &&
+              (lengths_out->data != lengths->data || N == 0),
+          "outputs must not be the inputs");
+  const int64_t need = 4 * (4 * N + 1);
+  NTB_ARG(workspace != nullptr && workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
+          (long long)workspace_bytes, (long long)need);
+  cudaStream_t st = (cudaStream_t)stream;
+  if ((rc = copy_refs(refs, refs_out, st)) != NTB_OK) return rc;
+  int* ws = reinterpret_cast<int*>(workspace);
+  a.out = reinterpret_cast<int*>(table_out->data);
+  a.lengths = reinterpret_cast<const int*>(lengths->data);
+  a.parents = reinterpret_cast<const int*>(parents->data);
+  a.len_s = lengths->stride[0];
+  a.par_s = parents->stride[0];
+  a.new_lengths = reinterpret_cast<int*>(lengths_out->data);
+  a.refs = reinterpret_cast<int*>(refs_out->data);
+  a.N = (int)N;
+  a.P = c.P;
+  a.T = c.T;
+  a.missing = reinterpret_cast<int*>(missing->data);
+  a.count = ws;
+  a.need = ws + 1;
+  a.want = a.need + N;
+  a.src = a.want + N;
+  a.dst = a.src + N;
+  const int rows = std::max(a.in.B, a.N);
+  if (rows > 0) {
+    reorder_rows_kernel<<<rows, 128, 0, st>>>(a);
+    NTB_LAUNCH_CHECK();
+  }
+  NTB_CUDA(launch_dependent(reorder_assign_kernel, dim3(1), dim3(kPlanThreads), 0, st, a));
+  c.src = a.src;
+  c.dst = a.dst;
+  c.src_s = c.dst_s = 1;
+  c.count = a.count;
+  c.pairs = a.N;
+  return launch_copy(c, st);
+}
+
+extern "C" int ntb_kv_compact(const NtbKvCache* cache, const NtbTensor* block_table, const NtbTensor* refs,
+                              const NtbTensor* table_out, const NtbTensor* refs_out, const NtbTensor* used,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace ntb;
+  using namespace ntb::kv;
+  CopyArgs c = {};
+  CompactArgs a = {};
+  int rc;
+  if ((rc = fill_copy(cache, &c)) != NTB_OK) return rc;
+  if ((rc = fill_table(block_table, "block_table", &a.in)) != NTB_OK) return rc;
+  if ((rc = check_i32(refs, 1, "refs")) != NTB_OK) return rc;
+  if ((rc = check_out(table_out, 2, "table_out")) != NTB_OK) return rc;
+  if ((rc = check_out(refs_out, 1, "refs_out")) != NTB_OK) return rc;
+  if ((rc = check_out(used, 1, "used")) != NTB_OK) return rc;
+  NTB_ARG(refs->shape[0] == c.P && refs_out->shape[0] == c.P, "refs must have one entry for each page");
+  NTB_ARG(same_shape(table_out, block_table) && used->shape[0] == 1, "outputs must be shaped like block_table and [1]");
+  NTB_ARG((refs_out->data != refs->data || c.P == 0) &&
+              (table_out->data != block_table->data || numel(block_table) == 0),
+          "outputs must not be the inputs");
+  const int64_t need = 4 * (3ll * c.P + 1);
+  NTB_ARG(workspace != nullptr && workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
+          (long long)workspace_bytes, (long long)need);
+  cudaStream_t st = (cudaStream_t)stream;
+  int* ws = reinterpret_cast<int*>(workspace);
+  a.out = reinterpret_cast<int*>(table_out->data);
+  a.refs = reinterpret_cast<const int*>(refs->data);
+  a.ref_s = refs->stride[0];
+  a.new_refs = reinterpret_cast<int*>(refs_out->data);
+  a.used = reinterpret_cast<int*>(used->data);
+  a.P = c.P;
+  a.count = ws;
+  a.map = ws + 1;
+  a.src = a.map + c.P;
+  a.dst = a.src + c.P;
+  compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
+  NTB_LAUNCH_CHECK();
+  const int64_t n = numel(block_table);
+  if (n > 0) {
+    const int64_t grid = std::min<int64_t>((n + 255) / 256, 4ll * sm_count());
+    NTB_CUDA(launch_dependent(compact_table_kernel, dim3((unsigned)grid), dim3(256), 0, st, a));
+  }
+  c.src = a.src;
+  c.dst = a.dst;
+  c.src_s = c.dst_s = 1;
+  c.count = a.count;
+  c.pairs = (int)(c.P / 2 + 1);  // no more movers than holes: at most half of the pages
+  return launch_copy(c, st);
+}

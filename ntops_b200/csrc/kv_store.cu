@@ -1,0 +1,274 @@
+// ntb_kv_store: quantises new keys and values into a paged 8-bit cache.
+//
+// For each (row b, head h, page) that receives new tokens, with a = max |x| over the page's new
+// elements (finite ones) and qmax the code's largest value:
+//   s_new = 2^e, the smallest power of two with a <= qmax * s_new (e clamped to [-100, 120])
+//   s     = max(s_old, s_new) if the page already holds tokens of this row, else s_new
+//   old codes become round(code * s_old / s) where s > s_old; new codes are round_sat(x / s).
+// One group of threads owns a (b, h, page) of the keys or of the values, so nothing is shared
+// between groups: no atomics, one launch.  The page's new elements are loaded once, as 16-byte
+// vectors kept in registers between the maximum and the rounding.
+#include <algorithm>
+#include <type_traits>
+
+#include "kv_cache.cuh"
+
+namespace ntb {
+namespace kv {
+namespace {
+
+struct StoreArgs {
+  Layer c;
+  Table table;
+  const void *key, *value;
+  int64_t k_b, k_h, k_s, k_d, v_b, v_h, v_s, v_d;  // input strides
+  const int *start, *counts;                       // counts may be null: S for every row
+  int64_t st_s, ct_s;
+  int B, S, cover;                                 // cover: pages that S tokens can touch
+  int64_t units;                                   // 2 * B * H * cover
+};
+
+constexpr int kHeld = 8;  // 16-byte vectors a thread keeps in registers
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;  // infinities and NaN do not set the scale
+}
+
+// GT: threads of a group (32 or a whole block).  VEC: input rows and codes allow vectors.
+template <typename T, int CODE, int GT, bool VEC>
+__global__ void __launch_bounds__(GT == 32 ? 128 : GT) store_kernel(StoreArgs a) {
+  constexpr int VE = VEC ? 16 / (int)sizeof(T) : 1;
+  constexpr int kThreads = GT == 32 ? 128 : GT;
+  using V = ew::Vec<T, VE>;
+  __shared__ float red[kThreads / 32];
+  const int64_t unit = (int64_t)blockIdx.x * (kThreads / GT) + (GT == 32 ? threadIdx.x / 32 : 0);
+  if (unit >= a.units) return;  // whole warps (GT 32) or no block (GT = block) leave here
+  const int lane = GT == 32 ? threadIdx.x % 32 : threadIdx.x;
+  const int which = (int)(unit & 1);
+  int64_t u = unit >> 1;
+  const int j = (int)(u % a.cover);
+  u /= a.cover;
+  const int h = (int)(u % a.c.H), b = (int)(u / a.c.H);
+  const int start = a.start[(int64_t)b * a.st_s];
+  const int n = a.counts == nullptr ? a.S : min(max(a.counts[(int64_t)b * a.ct_s], 0), a.S);
+  const int T_ = a.c.T, D = a.c.D;
+  if (start < 0) return;                              // a padding slot
+  const int m = start / T_ + j;                       // table column of this page
+  const int64_t p0 = (int64_t)m * T_;                 // position of the page's first token
+  const int64_t lo = max((int64_t)start, p0), hi = min((int64_t)start + n, p0 + T_);
+  if (lo >= hi) return;
+  const int page = page_of(a.table, a.c.P, b, m);
+  if (page < 0) return;
+  const int kept = (int)(lo - p0);                    // tokens of this row already in the page
+  const int rows = (int)(hi - lo);
+  const T* x = reinterpret_cast<const T*>(which ? a.value : a.key) + (int64_t)b * (which ? a.v_b : a.k_b) +
+               (int64_t)h * (which ? a.v_h : a.k_h) + (int64_t)(lo - start) * (which ? a.v_s : a.k_s);
+  const int64_t x_s = which ? a.v_s : a.k_s, x_d = which ? a.v_d : a.k_d;
+  uint8_t* codes = (which ? a.c.value : a.c.key) + (int64_t)page * (which ? a.c.v_p : a.c.k_p) +
+                   (int64_t)h * (which ? a.c.v_h : a.c.k_h);
+  const int64_t c_t = which ? a.c.v_t : a.c.k_t;
+  float* sp = (which ? a.c.value_scale : a.c.key_scale) + (int64_t)page * (which ? a.c.vs_p : a.c.ks_p) +
+              (int64_t)h * (which ? a.c.vs_h : a.c.ks_h);
+  const float s_old = kept > 0 ? *sp : 0.f;
+
+  const int vpr = D / VE;           // vectors of a row
+  const int total = rows * vpr;
+  auto load = [&](int i) -> V {
+    const int r = i / vpr, d = (i - r * vpr) * VE;
+    if constexpr (VEC) return ew::load_cs(reinterpret_cast<const V*>(x + (int64_t)r * x_s + d));
+    V v;
+    v.v[0] = x[(int64_t)r * x_s + (int64_t)d * x_d];
+    return v;
+  };
+  V held[kHeld];
+  float amax = 0.f;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (lane + k * GT < total) held[k] = load(lane + k * GT);
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (lane + k * GT < total)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) amax = fmaxf(amax, finite_abs(cvt<float>(held[k].v[e])));
+  for (int i = lane + kHeld * GT; i < total; i += GT) {  // pages larger than the registers hold
+    const V v = load(i);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) amax = fmaxf(amax, finite_abs(cvt<float>(v.v[e])));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if constexpr (GT > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, red[w]);
+  } else {
+    __syncwarp();
+  }
+  // every thread of the group has read s_old by now
+  const float s_new = pow2(scale_exp<CODE>(amax));
+  const float s = kept > 0 ? fmaxf(s_old, s_new) : s_new;
+  if (lane == 0 && s != s_old) *sp = s;
+  if (kept > 0 && s > s_old) {
+    const float ratio = s_old / s;
+    for (int i = lane; i < kept * D; i += GT) {
+      uint8_t* c = codes + (int64_t)(i / D) * c_t + i % D;
+      *c = encode1<CODE>(decode1<CODE>(*c) * ratio);
+    }
+  }
+  const float inv = 1.f / s;  // exact, as is every product with it: s is a power of two
+  auto put = [&](int i, const V& v) {
+    const int r = i / vpr, d = (i - r * vpr) * VE;
+    uint8_t* c = codes + (int64_t)(kept + r) * c_t + d;
+    if constexpr (VEC) {
+      uint32_t w[VE / 4];
+#pragma unroll
+      for (int e = 0; e < VE; e += 4)
+        w[e / 4] = encode4<CODE>(cvt<float>(v.v[e]) * inv, cvt<float>(v.v[e + 1]) * inv, cvt<float>(v.v[e + 2]) * inv,
+                                 cvt<float>(v.v[e + 3]) * inv);
+      if constexpr (VE == 8) *reinterpret_cast<uint2*>(c) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(c) = w[0];
+    } else {
+      *c = encode1<CODE>(cvt<float>(v.v[0]) * inv);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (lane + k * GT < total) put(lane + k * GT, held[k]);
+  for (int i = lane + kHeld * GT; i < total; i += GT) put(i, load(i));
+}
+
+template <typename T, int CODE, bool VEC>
+int launch_store(const StoreArgs& a, cudaStream_t st) {
+  // A warp a page while its registers hold the page's new elements, else a block.
+  const int64_t vecs = (int64_t)std::min(a.S, a.c.T) * (a.c.D / (VEC ? 16 / (int)sizeof(T) : 1));
+  const bool warp = vecs <= 32 * kHeld;
+  const int64_t grid = warp ? (a.units + 3) / 4 : a.units;
+  NTB_UNSUP(grid <= 0x7fffffffLL, "kv_store: too many pages in one call");
+  if (warp) store_kernel<T, CODE, 32, VEC><<<(unsigned)grid, 128, 0, st>>>(a);
+  else if (vecs <= 128 * kHeld) store_kernel<T, CODE, 128, VEC><<<(unsigned)grid, 128, 0, st>>>(a);
+  else store_kernel<T, CODE, 256, VEC><<<(unsigned)grid, 256, 0, st>>>(a);
+  NTB_LAUNCH_CHECK();
+  return NTB_OK;
+}
+
+template <typename T>
+int launch_typed(const StoreArgs& a, bool vec, cudaStream_t st) {
+  if (a.c.code == NTB_F8E4M3)
+    return vec ? launch_store<T, NTB_F8E4M3, true>(a, st) : launch_store<T, NTB_F8E4M3, false>(a, st);
+  return vec ? launch_store<T, NTB_I8, true>(a, st) : launch_store<T, NTB_I8, false>(a, st);
+}
+
+}  // namespace
+
+int check_i32(const NtbTensor* t, int ndim, const char* name) {
+  int rc = check_tensor(t, name);
+  if (rc != NTB_OK) return rc;
+  NTB_ARG(t->ndim == ndim, "%s must be %d-D, got %d-D", name, ndim, t->ndim);
+  NTB_UNSUP(t->dtype == NTB_I32, "%s must be int32, got %s", name, dtype_name(t->dtype));
+  return NTB_OK;
+}
+
+int check_cache(const NtbKvCache* c, bool layers, Layer* l) {
+  NTB_ARG(c != nullptr, "cache is NULL");
+  const NtbTensor* code[2] = {&c->key, &c->value};
+  const NtbTensor* scale[2] = {&c->key_scale, &c->value_scale};
+  const char* cn[2] = {"cache key", "cache value"};
+  const char* sn[2] = {"cache key_scale", "cache value_scale"};
+  const int off = layers ? 1 : 0, nd = 4 + off;
+  int rc;
+  for (int i = 0; i < 2; ++i) {
+    if ((rc = check_tensor(code[i], cn[i])) != NTB_OK) return rc;
+    if ((rc = check_tensor(scale[i], sn[i])) != NTB_OK) return rc;
+    NTB_ARG(code[i]->ndim == nd, "%s must be %d-D, got %d-D", cn[i], nd, code[i]->ndim);
+    NTB_UNSUP(code[i]->dtype == NTB_F8E4M3 || code[i]->dtype == NTB_I8, "%s must be float8_e4m3 or int8, got %s",
+              cn[i], dtype_name(code[i]->dtype));
+    NTB_ARG(code[i]->stride[nd - 1] == 1 || code[i]->shape[nd - 1] == 1, "%s must have a unit inner stride", cn[i]);
+    NTB_ARG(scale[i]->ndim == nd - 2, "%s must be %d-D, got %d-D", sn[i], nd - 2, scale[i]->ndim);
+    NTB_UNSUP(scale[i]->dtype == NTB_F32, "%s must be float32, got %s", sn[i], dtype_name(scale[i]->dtype));
+    for (int d = 0; d < nd - 2; ++d)
+      NTB_ARG(scale[i]->shape[d] == code[i]->shape[d], "%s and %s disagree at dim %d", sn[i], cn[i], d);
+    for (int d = 0; d < nd; ++d)
+      NTB_ARG(code[i]->shape[d] <= 0x7fffffffLL, "%s: dim %d is too large", cn[i], d);
+  }
+  NTB_UNSUP(c->key.dtype == c->value.dtype, "cache key and value must share one code type");
+  NTB_ARG(same_shape(&c->key, &c->value), "cache key and value shapes differ");
+  NTB_ARG(c->key.shape[off + 1] > 0 && c->key.shape[off + 2] > 0 && c->key.shape[off + 3] > 0,
+          "cache needs at least one head, token a page and channel");
+  NTB_ARG(c->key.shape[off + 2] * c->key.shape[off + 3] <= (1 << 30), "cache pages are too large");
+  l->key = reinterpret_cast<uint8_t*>(c->key.data);
+  l->value = reinterpret_cast<uint8_t*>(c->value.data);
+  l->key_scale = reinterpret_cast<float*>(c->key_scale.data);
+  l->value_scale = reinterpret_cast<float*>(c->value_scale.data);
+  l->k_p = c->key.stride[off]; l->k_h = c->key.stride[off + 1]; l->k_t = c->key.stride[off + 2];
+  l->v_p = c->value.stride[off]; l->v_h = c->value.stride[off + 1]; l->v_t = c->value.stride[off + 2];
+  l->ks_p = c->key_scale.stride[off]; l->ks_h = c->key_scale.stride[off + 1];
+  l->vs_p = c->value_scale.stride[off]; l->vs_h = c->value_scale.stride[off + 1];
+  l->P = (int)c->key.shape[off];
+  l->H = (int)c->key.shape[off + 1];
+  l->T = (int)c->key.shape[off + 2];
+  l->D = (int)c->key.shape[off + 3];
+  l->code = c->key.dtype;
+  return NTB_OK;
+}
+
+}  // namespace kv
+}  // namespace ntb
+
+extern "C" int ntb_kv_store(const NtbKvCache* cache, const NtbTensor* key, const NtbTensor* value,
+                            const NtbTensor* block_table, const NtbTensor* start, const NtbTensor* counts,
+                            void* stream) {
+  using namespace ntb;
+  using namespace ntb::kv;
+  StoreArgs a = {};
+  int rc;
+  if ((rc = check_cache(cache, false, &a.c)) != NTB_OK) return rc;
+  if ((rc = check_tensor(key, "key")) != NTB_OK) return rc;
+  if ((rc = check_tensor(value, "value")) != NTB_OK) return rc;
+  if ((rc = check_i32(block_table, 2, "block_table")) != NTB_OK) return rc;
+  if ((rc = check_i32(start, 1, "start")) != NTB_OK) return rc;
+  if (counts != nullptr && (rc = check_i32(counts, 1, "counts")) != NTB_OK) return rc;
+  NTB_ARG(key->ndim == 4 && same_shape(key, value), "key and value must be 4-D [B, H, S, D] of one shape");
+  NTB_UNSUP(key->dtype == value->dtype && (key->dtype == NTB_BF16 || key->dtype == NTB_F16 || key->dtype == NTB_F32),
+            "key and value must share one dtype: bfloat16, float16 or float32");
+  NTB_ARG(key->shape[1] == a.c.H && key->shape[3] == a.c.D, "key heads / head_dim differ from the cache's");
+  NTB_ARG(block_table->shape[0] == key->shape[0], "block_table rows differ from the batch");
+  NTB_ARG(start->shape[0] == key->shape[0], "start length differs from the batch");
+  NTB_ARG(counts == nullptr || counts->shape[0] == key->shape[0], "counts length differs from the batch");
+  NTB_ARG(key->shape[0] <= 0x7fffffffLL && key->shape[2] <= 0x7fffffffLL && block_table->shape[1] <= 0x7fffffffLL,
+          "kv_store: a dimension is too large");
+  a.B = (int)key->shape[0];
+  a.S = (int)key->shape[2];
+  a.table = {reinterpret_cast<const int*>(block_table->data), block_table->stride[0], block_table->stride[1], a.B,
+             (int)block_table->shape[1]};
+  if ((int64_t)a.B * a.S == 0 || a.c.P == 0 || a.table.M == 0) return NTB_OK;
+  a.key = key->data;
+  a.value = value->data;
+  a.k_b = key->stride[0]; a.k_h = key->stride[1]; a.k_s = key->stride[2]; a.k_d = key->stride[3];
+  a.v_b = value->stride[0]; a.v_h = value->stride[1]; a.v_s = value->stride[2]; a.v_d = value->stride[3];
+  a.start = reinterpret_cast<const int*>(start->data);
+  a.st_s = start->stride[0];
+  a.counts = counts ? reinterpret_cast<const int*>(counts->data) : nullptr;
+  a.ct_s = counts ? counts->stride[0] : 0;
+  a.cover = (int)std::min<int64_t>(((int64_t)a.S + a.c.T - 2) / a.c.T + 1, a.table.M);
+  a.units = 2ll * a.B * a.c.H * a.cover;
+  // vectors: 16-byte input rows; codes written 4 (fp32) or 8 (16-bit) at a time
+  const int es = dtype_size(key->dtype), ve = 16 / es;
+  auto in_ok = [&](const NtbTensor* t) {
+    return reinterpret_cast<uintptr_t>(t->data) % 16 == 0 && (t->stride[3] == 1) &&
+           (t->shape[0] == 1 || t->stride[0] % ve == 0) && (t->shape[1] == 1 || t->stride[1] % ve == 0) &&
+           (t->shape[2] == 1 || t->stride[2] % ve == 0);
+  };
+  auto out_ok = [&](const uint8_t* p, int64_t s0, int64_t s1, int64_t s2) {
+    return reinterpret_cast<uintptr_t>(p) % 8 == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
+  };
+  const bool vec = a.c.D % ve == 0 && in_ok(key) && in_ok(value) && out_ok(a.c.key, a.c.k_p, a.c.k_h, a.c.k_t) &&
+                   out_ok(a.c.value, a.c.v_p, a.c.v_h, a.c.v_t);
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (key->dtype) {
+    case NTB_BF16: return launch_typed<__nv_bfloat16>(a, vec, st);
+    case NTB_F16: return launch_typed<__half>(a, vec, st);
+    default: return launch_typed<float>(a, vec, st);
+  }
+}

@@ -47,7 +47,7 @@ unsigned int* device_error_ptr();
 // --------------------------------------------------------------- dtype helpers ------------
 inline int dtype_size(int dt) {
   switch (dt) {
-    case NTB_BOOL: case NTB_U8: case NTB_I8: return 1;
+    case NTB_BOOL: case NTB_U8: case NTB_I8: case NTB_F8E4M3: return 1;
     case NTB_I16: case NTB_F16: case NTB_BF16: return 2;
     case NTB_I32: case NTB_F32: return 4;
     case NTB_I64: case NTB_F64: return 8;

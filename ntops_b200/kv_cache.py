@@ -1,0 +1,248 @@
+"""A paged KV cache held in 8 bits, with the operators a serving loop runs on it (beyond the
+reference's operator list, whose KV cache is a contiguous tensor in the model's type).
+
+``PagedKVCache`` holds, for all layers, the codes of keys and values in pages of ``page_size``
+tokens (``torch.float8_e4m3fn`` or ``torch.int8``) and one fp32 scale for each (page, kv head):
+value = code * scale.  A block table, int32 [B, M], names for each row (sequence) the page of
+tokens [m * page_size, (m + 1) * page_size); a negative entry is a hole.  ``refs``, int32 [P],
+counts how often each page is referenced; 0 = free.  One block table serves all layers.
+
+    cache = PagedKVCache.allocate(layers, pages, kv_heads, page_size, head_dim)
+    table, refs, missing = extend(cache, table, refs, lengths + new)     # pages for new tokens
+    store(cache.layer(i), k, v, table, start=lengths)                    # quantise them
+    o = attention(q, cache.layer(i), table, lengths + new)               # attend over them
+    table, lengths, refs, missing = reorder(cache, table, lengths, refs, parents)  # fork / free
+    table, refs, used = compact(cache, table, refs)                      # used pages to the front
+    copy_pages(cache, src, dst)
+
+Nothing here waits for the GPU: lengths, tables and counts stay on the device, and what did not
+fit comes back as a count on the device too.  All calls run on the current stream of the cache's
+device.  ``attention`` gives zeros to a query that sees no key.
+"""
+
+import ctypes
+import math
+
+import torch
+
+from ntops_b200 import _lib
+from ntops_b200.torch.utils import _check_cuda, launch, lib
+
+_CODES = {torch.float8_e4m3fn: 10, torch.int8: _lib.DTYPE_CODES[torch.int8]}
+_QUERY_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_DIMS = ctypes.c_int64 * _lib.MAX_DIMS
+
+
+def _desc(t, code):
+    return _lib.NtbTensor(t.data_ptr(), code, t.dim(), _DIMS(*t.shape), _DIMS(*t.stride()))
+
+
+def _tensor(t, name, device, dtypes, ndim):
+    """Descriptor of an operand after the checks that need Python's view of it."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.device != device:
+        _check_cuda(t)
+        raise RuntimeError(f"{name} is on {t.device}, the cache on {device}")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.dim() != ndim:
+        raise RuntimeError(f"{name} must be {ndim}-D, got {t.dim()}-D")
+    return _desc(t, _lib.DTYPE_CODES[t.dtype])
+
+
+_I32 = (torch.int32,)
+
+
+class _CacheView:
+    """The cache's tensors with the descriptors that the kernels read them through."""
+
+    def __init__(self, key, value, key_scale, value_scale):
+        self.key, self.value, self.key_scale, self.value_scale = key, value, key_scale, value_scale
+        self.device = key.device
+        self._c = _lib.NtbKvCache(_desc(key, _CODES[key.dtype]), _desc(value, _CODES[value.dtype]),
+                                  _desc(key_scale, _lib.DTYPE_CODES[torch.float32]),
+                                  _desc(value_scale, _lib.DTYPE_CODES[torch.float32]))
+        self._ref = ctypes.byref(self._c)
+
+
+class PagedKVLayer(_CacheView):
+    """One layer of a ``PagedKVCache``: key, value [P, H, page, D], key_scale, value_scale [P, H]."""
+
+
+class PagedKVCache(_CacheView):
+    """key, value: codes [layers, pages, kv_heads, page_size, head_dim], any strides with a unit
+    inner one (so [layers, pages, page_size, kv_heads, head_dim] storage passes as a transposed
+    view); key_scale, value_scale: fp32 [layers, pages, kv_heads].  The tensors are used as they
+    are, not copied."""
+
+    def __init__(self, key, value, key_scale, value_scale):
+        for name, t in (("key", key), ("value", value), ("key_scale", key_scale), ("value_scale", value_scale)):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+        _check_cuda(key, value, key_scale, value_scale)
+        if not key.device == value.device == key_scale.device == value_scale.device:
+            raise RuntimeError("the cache's tensors must share one device")
+        if key.dtype not in _CODES or value.dtype != key.dtype:
+            raise RuntimeError(f"key and value must both be float8_e4m3fn or int8, got {key.dtype} and {value.dtype}")
+        if key.dim() != 5 or value.shape != key.shape:
+            raise RuntimeError("key and value must be [layers, pages, kv_heads, page_size, head_dim] of one shape")
+        if key_scale.dtype != torch.float32 or value_scale.dtype != torch.float32:
+            raise RuntimeError("key_scale and value_scale must be float32")
+        if key_scale.shape != key.shape[:3] or value_scale.shape != key.shape[:3]:
+            raise RuntimeError("key_scale and value_scale must be [layers, pages, kv_heads]")
+        if any(t.shape[-1] > 1 and t.stride(-1) != 1 for t in (key, value)):
+            raise RuntimeError("key and value must have a unit inner stride")
+        super().__init__(key, value, key_scale, value_scale)
+        self._layers = [PagedKVLayer(key[i], value[i], key_scale[i], value_scale[i]) for i in range(key.shape[0])]
+
+    @classmethod
+    def allocate(cls, layers, pages, kv_heads, page_size, head_dim, dtype=torch.float8_e4m3fn, device="cuda"):
+        """A cache of zeros."""
+        if dtype not in _CODES:
+            raise RuntimeError(f"dtype must be float8_e4m3fn or int8, got {dtype}")
+        shape = (layers, pages, kv_heads, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for _ in range(2))
+        ks, vs = (torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs)
+
+    @property
+    def page_size(self):
+        return self.key.shape[3]
+
+    @property
+    def num_pages(self):
+        return self.key.shape[1]
+
+    @property
+    def num_layers(self):
+        return self.key.shape[0]
+
+    def layer(self, i):
+        return self._layers[i]
+
+
+def _view(cache, kind, what):
+    if not isinstance(cache, kind):
+        hint = " (cache.layer(i))" if kind is PagedKVLayer else ""
+        raise TypeError(f"{what} takes a {kind.__name__}{hint}, got {type(cache).__name__}")
+    return cache
+
+
+def store(layer, key, value, block_table, start, counts=None):
+    """Quantises key, value [B, H, S, D] (bf16, fp16 or fp32; any strides) into the layer's pages:
+    token i of row b goes to position start[b] + i, for i < counts[b] (default S).  Rows with a
+    negative start, tokens past the table and tokens in holes are dropped.
+
+    For each page and head, with a = max |x| over the page's new elements (finite ones) and qmax the
+    code's largest value (448 or 127), s_new is the smallest power of two with a <= qmax * s_new.
+    If the page holds earlier tokens of the row the scale becomes max(s_old, s_new) and, where it
+    grows, their codes are re-rounded (for e4m3 that changes values in the code's subnormal range
+    only); else it becomes s_new.  Codes round to nearest even and saturate.  Two rows must not
+    store into the same page: ``reorder`` gives forked rows pages of their own to go on in."""
+    c = _view(layer, PagedKVLayer, "store")
+    kd = _tensor(key, "key", c.device, _QUERY_TYPES, 4)
+    vd = _tensor(value, "value", c.device, _QUERY_TYPES, 4)
+    td = _tensor(block_table, "block_table", c.device, _I32, 2)
+    sd = _tensor(start, "start", c.device, _I32, 1)
+    nd = None if counts is None else _tensor(counts, "counts", c.device, _I32, 1)
+    launch("kv_store", lib().ntb_kv_store, c._ref, kd, vd, td, sd, nd, device_tensor=c.key)
+
+
+def attention(query, layer, block_table, lengths, scale=None, is_causal=True, start=None):
+    """Attention of query [B, Hq, Sq, D] over the layer's tokens; returns [B, Hq, Sq, D] in the
+    query's type and memory layout.
+
+    Row b's query i stands at position start[b] + i (default lengths[b] - Sq: the queries are the
+    last tokens) and sees the keys before lengths[b], those past its position excepted when
+    ``is_causal``, and those in holes.  kv head = query head // (Hq // H).  scale: 1 / sqrt(D) by
+    default.  A query that sees no key gives zeros.  Softmax statistics and sums are in fp32."""
+    c = _view(layer, PagedKVLayer, "attention")
+    qd = _tensor(query, "query", c.device, _QUERY_TYPES, 4)
+    td = _tensor(block_table, "block_table", c.device, _I32, 2)
+    ld = _tensor(lengths, "lengths", c.device, _I32, 1)
+    sd = None if start is None else _tensor(start, "start", c.device, _I32, 1)
+    if query.shape[-1] > 1 and query.stride(-1) != 1:
+        raise RuntimeError("query must have a unit inner stride")
+    if scale is None:
+        scale = 1 / math.sqrt(query.shape[-1])
+    L = lib()
+    nbytes = ctypes.c_int64(0)
+    with _lib.device_of(query):
+        _lib.check(L.ntb_kv_attention_workspace(qd, c._ref, td, ctypes.byref(nbytes)), "kv_attention")
+    output = torch.empty_like(query)
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=c.device)
+    launch("kv_attention", L.ntb_kv_attention, qd, c._ref, td, ld, sd, _desc(output, qd.dtype), float(scale),
+           int(bool(is_causal)), ctypes.c_void_p(ws.data_ptr()), nbytes.value, device_tensor=output)
+    return output
+
+
+def copy_pages(cache, src, dst):
+    """Copies pages src[k] to dst[k] (int32 [n]) with their scales, in every layer.  No page may be
+    both a source and a destination, nor twice a destination; pairs out of range are skipped."""
+    c = _view(cache, PagedKVCache, "copy_pages")
+    sd, dd = _tensor(src, "src", c.device, _I32, 1), _tensor(dst, "dst", c.device, _I32, 1)
+    launch("kv_copy_pages", lib().ntb_kv_copy_pages, c._ref, sd, dd, device_tensor=c.key)
+
+
+def _refs(refs, c):
+    d = _tensor(refs, "refs", c.device, _I32, 1)
+    if refs.shape[0] != c.num_pages:
+        raise RuntimeError(f"refs has {refs.shape[0]} entries, the cache {c.num_pages} pages")
+    if not refs.is_contiguous():
+        raise RuntimeError("refs must be contiguous")
+    return d
+
+
+def extend(cache, block_table, refs, lengths):
+    """Gives every entry of the block table that lengths[b] tokens need and that holds no page the
+    lowest-numbered free page, in row order.  Returns ``(block_table, refs, missing)``, new tensors;
+    missing, int32 [1], counts entries that found no free page and stay holes."""
+    c = _view(cache, PagedKVCache, "extend")
+    td, rd = _tensor(block_table, "block_table", c.device, _I32, 2), _refs(refs, c)
+    ld = _tensor(lengths, "lengths", c.device, _I32, 1)
+    table = torch.empty(block_table.shape, dtype=torch.int32, device=c.device)
+    out, missing = torch.empty_like(refs), torch.empty(1, dtype=torch.int32, device=c.device)
+    ws = torch.empty(max(block_table.numel(), 1), dtype=torch.int32, device=c.device)
+    launch("kv_extend", lib().ntb_kv_extend, td, ld, rd, c.page_size, _desc(table, td.dtype), _desc(out, td.dtype),
+           _desc(missing, td.dtype), ctypes.c_void_p(ws.data_ptr()), 4 * ws.numel(), device_tensor=c.key)
+    return table, out, missing
+
+
+def reorder(cache, block_table, lengths, refs, parents):
+    """Makes new row i continue old row parents[i] (int32 [N]; an index outside the batch makes an
+    empty row): forks rows that are named several times (parallel samples, beams), frees rows that
+    are not named, permutes the others.
+
+    Full pages are shared.  The first new row that continues an old one keeps its partly filled last
+    page (and any reserved after it); each further one gets a copy of that page, in all layers, in
+    the lowest-numbered page that is free once the old rows' references are gone.  Returns
+    ``(block_table [N, M], lengths [N], refs, missing)``, new tensors; missing, int32 [1], counts
+    copies that found no free page (their entries are holes: take pages back before going on)."""
+    c = _view(cache, PagedKVCache, "reorder")
+    td, rd = _tensor(block_table, "block_table", c.device, _I32, 2), _refs(refs, c)
+    ld, pd = _tensor(lengths, "lengths", c.device, _I32, 1), _tensor(parents, "parents", c.device, _I32, 1)
+    n = parents.shape[0]
+    table = torch.empty((n, block_table.shape[1]), dtype=torch.int32, device=c.device)
+    lens, out = torch.empty(n, dtype=torch.int32, device=c.device), torch.empty_like(refs)
+    missing = torch.empty(1, dtype=torch.int32, device=c.device)
+    ws = torch.empty(4 * n + 1, dtype=torch.int32, device=c.device)
+    i32 = td.dtype
+    launch("kv_reorder", lib().ntb_kv_reorder, c._ref, td, ld, rd, pd, _desc(table, i32), _desc(lens, i32),
+           _desc(out, i32), _desc(missing, i32), ctypes.c_void_p(ws.data_ptr()), 4 * ws.numel(), device_tensor=c.key)
+    return table, lens, out, missing
+
+
+def compact(cache, block_table, refs):
+    """Moves the used pages (refs > 0) to the front of the pool, in all layers: with U of them in use,
+    the k-th used page past the first U moves to the k-th free page among them.  Returns
+    ``(block_table, refs, used)``, new tensors; used, int32 [1], is U: pages from U on are free."""
+    c = _view(cache, PagedKVCache, "compact")
+    td, rd = _tensor(block_table, "block_table", c.device, _I32, 2), _refs(refs, c)
+    table = torch.empty(block_table.shape, dtype=torch.int32, device=c.device)
+    out, used = torch.empty_like(refs), torch.empty(1, dtype=torch.int32, device=c.device)
+    ws = torch.empty(3 * c.num_pages + 1, dtype=torch.int32, device=c.device)
+    i32 = td.dtype
+    launch("kv_compact", lib().ntb_kv_compact, c._ref, td, rd, _desc(table, i32), _desc(out, i32), _desc(used, i32),
+           ctypes.c_void_p(ws.data_ptr()), 4 * ws.numel(), device_tensor=c.key)
+    return table, out, used

@@ -1,0 +1,164 @@
+"""Plain 64-bit restatement of the paged 8-bit KV cache operators (CPU, row by row).
+
+Codes are handled as the values they stand for; ``round_code`` rounds to a code's values from the
+formats' definitions (e4m3: 3 mantissa bits, exponents from -6, subnormal step 2^-9, largest 448;
+int8: integers within +-127).
+"""
+
+import math
+
+import torch
+
+QMAX = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
+
+
+def round_code(y, dtype):
+    """fp64 values -> fp64 values of the code: nearest, ties to even, saturating."""
+    top = QMAX[dtype]
+    if dtype == torch.int8:
+        return torch.nan_to_num(y, nan=0.0).round().clamp(-top, top)
+    y = y.clamp(-top, top)
+    e = torch.floor(torch.log2(y.abs().clamp(min=2.0**-20))).clamp(min=-6)
+    step = torch.exp2(e - 3)
+    return ((y / step).round() * step).clamp(-top, top)
+
+
+def scale_of(amax, dtype):
+    """The smallest power of two s, within [2^-100, 2^120], with amax <= qmax * s."""
+    if amax == 0:
+        return 2.0**-100
+    e = math.ceil(math.log2(amax / QMAX[dtype]))
+    while e > -100 and amax <= QMAX[dtype] * 2.0 ** (e - 1):
+        e -= 1
+    while amax > QMAX[dtype] * 2.0**e:
+        e += 1
+    return 2.0 ** min(max(e, -100), 120)
+
+
+def store(codes, scales, new, table, start, counts, dtype):
+    """codes fp64 [P, H, T, D], scales fp64 [P, H] (updated in place); new [B, H, S, D]."""
+    P, H, T, D = codes.shape
+    for b in range(new.shape[0]):
+        n = new.shape[2] if counts is None else min(max(int(counts[b]), 0), new.shape[2])
+        s0 = int(start[b])
+        if s0 < 0:
+            continue
+        for m in range(table.shape[1]):
+            lo, hi = max(m * T, s0), min((m + 1) * T, s0 + n)
+            p = int(table[b, m])
+            if lo >= hi or not 0 <= p < P:
+                continue
+            kept = lo - m * T
+            for h in range(H):
+                x = new[b, h, lo - s0:hi - s0].double()
+                fin = x[torch.isfinite(x)]
+                s = scale_of(float(fin.abs().max()) if fin.numel() else 0.0, dtype)
+                if kept:
+                    old = float(scales[p, h])
+                    s = max(s, old)
+                    if s > old:
+                        codes[p, h, :kept] = round_code(codes[p, h, :kept] * (old / s), dtype)
+                scales[p, h] = s
+                codes[p, h, kept:kept + hi - lo] = round_code(x / s, dtype)
+
+
+def attention(q, key, value, key_scale, value_scale, table, lengths, scale, causal, start=None):
+    """q [B, Hq, Sq, D]; key, value fp64 code values [P, H, T, D]; scales fp64 [P, H].  Returns
+    (out, bound): fp64 outputs and, for error bounds, the pair (sum_j p_j |v_j|, largest
+    scale * sum_d |q_d k_jd|) of each output row."""
+    B, Hq, Sq, D = q.shape
+    P, H, T, _ = key.shape
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    mag = torch.zeros(q.shape, dtype=torch.float64)
+    dots = torch.zeros(q.shape[:3], dtype=torch.float64)
+    for b in range(B):
+        n = min(max(int(lengths[b]), 0), table.shape[1] * T)
+        s0 = n - Sq if start is None else int(start[b])
+        at = [(int(table[b, j // T]), j % T, j) for j in range(n)]
+        at = [(p, t, j) for p, t, j in at if 0 <= p < P]
+        if not at:
+            continue
+        p, t, j = (torch.tensor(x) for x in zip(*at))
+        for h in range(Hq):
+            g = h // (Hq // H)
+            k = key[p, g, t] * key_scale[p, g].view(-1, 1)
+            v = value[p, g, t] * value_scale[p, g].view(-1, 1)
+            for i in range(Sq):
+                seen = j <= s0 + i if causal else torch.ones_like(j, dtype=torch.bool)
+                if not seen.any():
+                    continue
+                x = q[b, h, i].double()
+                w = torch.softmax(k[seen] @ x * scale, 0)
+                out[b, h, i] = w @ v[seen]
+                mag[b, h, i] = w @ v[seen].abs()
+                dots[b, h, i] = (k[seen].abs() @ x.abs()).max() * abs(scale)
+    return out, (mag, dots)
+
+
+def extend(table, lengths, refs, page_size):
+    table, refs = table.clone(), refs.clone()
+    missing = 0
+    for b in range(table.shape[0]):
+        for m in range(table.shape[1]):
+            if not 0 <= int(table[b, m]) < refs.numel():
+                table[b, m] = -1
+                if m * page_size < int(lengths[b]):
+                    free = (refs == 0).nonzero()
+                    if free.numel():
+                        table[b, m] = int(free[0])
+                        refs[free[0]] = 1
+                    else:
+                        missing += 1
+    return table, refs, missing
+
+
+def reorder(table, lengths, refs, parents, page_size):
+    """Returns (table, lengths, refs, missing, copies): copies is a list of (src, dst) pages."""
+    B, M = table.shape
+    P, N = refs.numel(), parents.numel()
+    refs = refs.clone()
+    ok = lambda p: 0 <= int(p) < P  # noqa: E731
+    for p in table.reshape(-1):
+        if ok(p):
+            refs[p] -= 1
+    new, lens = torch.full((N, M), -1, dtype=torch.int32), torch.zeros(N, dtype=torch.int32)
+    want, seen = [], set()
+    for i, b in enumerate(parents.tolist()):
+        if not 0 <= b < B:
+            continue
+        lens[i] = max(int(lengths[b]), 0)
+        whole, part = divmod(int(lens[i]), page_size)
+        for m in range(M):
+            if not ok(table[b, m]):
+                continue
+            if b not in seen or m < whole:
+                new[i, m] = table[b, m]
+                refs[table[b, m]] += 1
+            elif m == whole and part:
+                want.append((i, m, int(table[b, m])))
+        seen.add(b)
+    copies, missing = [], 0
+    free = (refs == 0).nonzero().view(-1).tolist()
+    for k, (i, m, src) in enumerate(want):
+        if k < len(free):
+            new[i, m] = free[k]
+            refs[free[k]] = 1
+            copies.append((src, free[k]))
+        else:
+            missing += 1
+    return new, lens, refs, missing, copies
+
+
+def compact(table, refs):
+    """Returns (table, refs, used, moves)."""
+    P = refs.numel()
+    used = [p for p in range(P) if refs[p] > 0]
+    U = len(used)
+    moves = list(zip([p for p in used if p >= U], [p for p in range(U) if refs[p] <= 0]))
+    to = {p: p for p in used}
+    to.update(dict(moves))
+    new = torch.tensor([[to.get(int(p), -1) for p in row] for row in table], dtype=torch.int32).view(table.shape)
+    out = torch.zeros_like(refs)
+    for p in used:
+        out[to[p]] = refs[p]
+    return new, out, U, moves

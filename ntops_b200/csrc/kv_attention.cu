@@ -276,6 +276,7 @@ int fill(const NtbTensor* q, const NtbKvCache* cache, const NtbTensor* table, At
 int plan(AttnArgs* a, int dtype) {
   a->b0 = 0;
   a->nb = std::min(a->table.B, kMaxBatch);
+  if (decode_takes(*a, dtype)) return decode_plan(a, dtype);
   a->tile = kGenTile;
   a->unit = kGenUnit;
   a->tiles = (a->rows + a->tile - 1) / a->tile;
@@ -337,7 +338,8 @@ extern "C" int ntb_kv_attention(const NtbTensor* q, const NtbKvCache* cache, con
   NTB_UNSUP((int64_t)kMaxBatch * a.tiles * a.c.H <= 0x7fffffffLL, "kv_attention: too many query rows");
   for (a.b0 = 0; a.b0 < a.table.B; a.b0 += kMaxBatch) {
     a.nb = std::min(a.table.B - a.b0, kMaxBatch);
-    if ((rc = generic_any(a, q->dtype, st, nullptr)) != NTB_OK) return rc;
+    rc = decode_takes(a, q->dtype) ? decode_launch(a, q->dtype, st) : generic_any(a, q->dtype, st, nullptr);
+    if (rc != NTB_OK) return rc;
     if ((rc = combine_launch(a, q->dtype, st)) != NTB_OK) return rc;
   }
   return NTB_OK;

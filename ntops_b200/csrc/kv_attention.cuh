@@ -19,7 +19,7 @@ namespace ntb {
 namespace kv {
 
 constexpr float kLog2eF = 1.4426950408889634f;
-constexpr int kMaxBatch = 4096;  // batch rows of one launch (their unit counts sit in shared memory)
+constexpr int kMaxBatch = 2048;  // batch rows of one launch (their unit counts sit in shared memory)
 
 struct AttnArgs {
   const void* q;

@@ -236,7 +236,7 @@ def test_attention_many_rows():
     n = torch.randint(0, 60, (b,), dtype=torch.int32)
     q = torch.randn(b, 2, 1, 64).to(BF16)
     got = kc.attention(q.to(DEV), cache.layer(0), table.to(DEV), n.to(DEV))
-    pick = torch.tensor([0, 1, 2, 77, 4094, 4095, 4096, 4097, 4099])
+    pick = torch.tensor([0, 1, 2, 77, 2047, 2048, 4094, 4095, 4096, 4097, 4099])
     _check_attention(got[pick.to(DEV)], q[pick], cache, 0, table[pick], n[pick], 0.125, True)
 
 

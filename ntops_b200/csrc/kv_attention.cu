@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(kGenThreads) generic_kernel(AttnArgs a) {
   __shared__ int ids[kGenKeys];
   __shared__ float ksc[kGenKeys], vsc[kGenKeys];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_launch();  // the joining kernel may start; it waits for this one before it reads
   prefix_units<kGenThreads>(a, pre);
   const Line line(a, pre);
   if ((int)blockIdx.x >= line.blocks) return;
@@ -138,55 +139,99 @@ __global__ void __launch_bounds__(kGenThreads) generic_kernel(AttnArgs a) {
         for (int c = 0; c < DC; ++c)
           if (lane + 32 * c < D) o[lane + 32 * c] = cvt<T>(l[i] == 0.f ? 0.f : acc[i][c] * inv);
       } else {
-        float* w = a.part + (int64_t)pc.slot * slot_floats(a.tile, D) + (int64_t)rt * (D + 2);
+        float* w = a.part + (int64_t)pc.slot * slot_floats(a.tile, D);
 #pragma unroll
         for (int c = 0; c < DC; ++c)
-          if (lane + 32 * c < D) w[lane + 32 * c] = acc[i][c];
+          if (lane + 32 * c < D) w[(int64_t)rt * D + lane + 32 * c] = acc[i][c];
         if (lane == 0) {
-          w[D] = m[i];
-          w[D + 1] = l[i];
+          w[(int64_t)a.tile * D + 2 * rt] = m[i];
+          w[(int64_t)a.tile * D + 2 * rt + 1] = l[i];
         }
       }
     }
   }
 }
 
-// Joins the pieces of every cut segment, one block a segment:
+// Joins the pieces of every cut segment, one warp a row:
 //   M = max_c m_c,  out = sum_c O_c 2^(m_c - M) / sum_c l_c 2^(m_c - M).
-template <typename T>
-__global__ void __launch_bounds__(128) combine_kernel(AttnArgs a) {
+// Lanes hold the statistics of 32 pieces at a time and then the row's channels; the loads of
+// eight pieces are in flight together.
+constexpr int kCombineWarps = 4;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(AttnArgs a) {
+  constexpr int E = VEC ? 4 : 1;    // channels of a lane at a time
+  constexpr int N = VEC ? 2 : 8;    // head_dim <= 256 = 32 * E * N
+  using V = ew::Vec<float, E>;
   extern __shared__ int pre[];
-  prefix_units<128>(a, pre);  // lengths are inputs of the whole call, not of the previous kernel
+  prefix_units<32 * kCombineWarps>(a, pre);  // lengths are the call's inputs, not the previous kernel's output
   const Line line(a, pre);
-  const int x = blockIdx.x / line.segs, seg = blockIdx.x % line.segs;
+  const int lane = threadIdx.x & 31;
+  const int64_t job = (int64_t)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
+  const int rt = (int)(job % a.tile);
+  const int64_t sg = job / a.tile;
+  const int x = (int)(sg / line.segs), seg = (int)(sg % line.segs);
+  if (x >= a.nb) return;
+  const int tile = seg / a.c.H, head = seg % a.c.H, r = tile * a.tile + rt;
+  if (r >= a.rows) return;
   const int units = pre[x + 1] - pre[x];
   const int64_t u0 = (int64_t)pre[x] * line.segs + (int64_t)seg * units;
   const int c0 = line.owner(u0), c1 = line.owner(u0 + units - 1);
-  grid_dependency_wait();
   if (c0 == c1) return;  // whole: its block wrote the output
-  const int D = a.c.D, b = a.b0 + x, tile = seg / a.c.H, head = seg % a.c.H;
-  for (int rt = 0; rt < a.tile; ++rt) {
-    const int r = tile * a.tile + rt;
-    if (r >= a.rows) break;
-    const float* first = a.part + (int64_t)(2 * c0 + (line.begin(c0) < u0 ? 1 : 0)) * slot_floats(a.tile, D) +
-                         (int64_t)rt * (D + 2);
-    const float* rest = a.part + (int64_t)rt * (D + 2);
-    auto piece = [&](int c) { return c == c0 ? first : rest + (int64_t)2 * c * slot_floats(a.tile, D); };
-    float M = -INFINITY;
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, piece(c)[D]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    T* o = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_b + (int64_t)(head * a.group + r % a.group) * a.o_h +
-           (int64_t)(r / a.group) * a.o_s;
-    for (int d = threadIdx.x; d < D; d += 128) {
-      float L = 0.f, acc = 0.f;
-      for (int c = c0; c <= c1; ++c) {
-        const float* w = piece(c);
-        const float f = exp2f(w[D] - ref);
-        L = fmaf(w[D + 1], f, L);
-        acc = fmaf(w[d], f, acc);
-      }
-      o[d] = cvt<T>(L == 0.f ? 0.f : acc / L);
+  const int D = a.c.D, b = a.b0 + x;
+  const int64_t slot = slot_floats(a.tile, D);
+  const int first = 2 * c0 + (line.begin(c0) < u0 ? 1 : 0);
+  auto piece = [&](int c) { return a.part + (int64_t)(c == c0 ? first : 2 * c) * slot; };
+  const int64_t stat = (int64_t)a.tile * D + 2 * rt;  // of the row's max and sum in a slot
+  grid_dependency_wait();
+  float M = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, piece(c)[stat]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float ref = M == -INFINITY ? 0.f : M;
+  float L = 0.f, acc[N][E];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[i][e] = 0.f;
+  for (int cb = c0; cb <= c1; cb += 32) {
+    float f = 0.f;
+    if (cb + lane <= c1) {
+      const float* w = piece(cb + lane) + stat;
+      f = exp2f(w[0] - ref);
+      L = fmaf(w[1], f, L);
     }
+    const int n = min(32, c1 - cb + 1);
+    for (int k0 = 0; k0 < n; k0 += 8) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int d = (lane + 32 * i) * E;
+        if (32 * i * E >= D) break;  // the same for the whole warp
+        V v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k0 + k < n && d < D) v[k] = *reinterpret_cast<const V*>(piece(cb + k0 + k) + (int64_t)rt * D + d);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float fk = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
+          if (k0 + k < n && d < D)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[i][e] = fmaf(v[k].v[e], fk, acc[i][e]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* o = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_b + (int64_t)(head * a.group + r % a.group) * a.o_h +
+         (int64_t)(r / a.group) * a.o_s;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = (lane + 32 * i) * E;
+    if (d < D)
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[d + e] = cvt<T>(L == 0.f ? 0.f : acc[i][e] * inv);
   }
 }
 
@@ -229,16 +274,18 @@ int generic_any(const AttnArgs& a, int dtype, cudaStream_t st, int* blocks) {
 int combine_launch(const AttnArgs& a, int dtype, cudaStream_t st) {
   // One unit for every segment at most: nothing can be cut.
   if ((int64_t)a.table.M * a.c.T <= a.unit) return NTB_OK;
-  const int64_t grid = (int64_t)a.nb * a.tiles * a.c.H;
+  const int64_t jobs = (int64_t)a.nb * a.tiles * a.c.H * a.tile, grid = (jobs + kCombineWarps - 1) / kCombineWarps;
   const size_t smem = sizeof(int) * (a.nb + 1);
+  NTB_UNSUP(grid <= 0x7fffffffLL, "kv_attention: too many query rows");
+  const bool vec = a.c.D % 4 == 0;
   auto go = [&](auto k) -> int {
-    NTB_CUDA(launch_dependent(k, dim3((unsigned)grid), dim3(128), smem, st, a));
+    NTB_CUDA(launch_dependent(k, dim3((unsigned)grid), dim3(32 * kCombineWarps), smem, st, a));
     return NTB_OK;
   };
   switch (dtype) {
-    case NTB_BF16: return go(combine_kernel<__nv_bfloat16>);
-    case NTB_F16: return go(combine_kernel<__half>);
-    default: return go(combine_kernel<float>);
+    case NTB_BF16: return vec ? go(combine_kernel<__nv_bfloat16, true>) : go(combine_kernel<__nv_bfloat16, false>);
+    case NTB_F16: return vec ? go(combine_kernel<__half, true>) : go(combine_kernel<__half, false>);
+    default: return vec ? go(combine_kernel<float, true>) : go(combine_kernel<float, false>);
   }
 }
 
@@ -335,7 +382,6 @@ extern "C" int ntb_kv_attention(const NtbTensor* q, const NtbKvCache* cache, con
   NTB_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
   a.part = reinterpret_cast<float*>(workspace);
   cudaStream_t st = (cudaStream_t)stream;
-  NTB_UNSUP((int64_t)kMaxBatch * a.tiles * a.c.H <= 0x7fffffffLL, "kv_attention: too many query rows");
   for (a.b0 = 0; a.b0 < a.table.B; a.b0 += kMaxBatch) {
     a.nb = std::min(a.table.B - a.b0, kMaxBatch);
     rc = decode_takes(a, q->dtype) ? decode_launch(a, q->dtype, st) : generic_any(a, q->dtype, st, nullptr);

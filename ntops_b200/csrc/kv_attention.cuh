@@ -36,7 +36,7 @@ struct AttnArgs {
   int tile, tiles;   // rows of a tile, tiles of a segment row
   int unit;          // keys of a unit
   int G;             // blocks that share the work
-  float* part;       // [2 * G][tile][D + 2]: O, then max (base 2), sum
+  float* part;       // [2 * G] slots: O [tile][D], then [tile] pairs of max (base 2) and sum
   unsigned int* err; // device error word (bounded waits)
 };
 

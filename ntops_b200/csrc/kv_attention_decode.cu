@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
   __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
+  grid_dependency_launch();  // the joining kernel may start; it waits for this one before it reads
   prefix_units<kThreads>(a, pre);
   const Line line(a, pre);
   if ((int)blockIdx.x >= line.blocks) return;
@@ -381,11 +382,11 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
         reinterpret_cast<T*>(a.o)[(int64_t)pc.b * a.o_b + (int64_t)(pc.head * a.group + r % a.group) * a.o_h +
                                   (int64_t)(r / a.group) * a.o_s + d] = cvt<T>(L == 0.f ? 0.f : acc / L);
       } else {
-        float* part = a.part + (int64_t)pc.slot * slot_floats(a.tile, D) + (int64_t)rt * (D + 2);
-        part[d] = acc;
+        float* part = a.part + (int64_t)pc.slot * slot_floats(a.tile, D);
+        part[rt * D + d] = acc;
         if (d == 0) {
-          part[D] = M;
-          part[D + 1] = L;
+          part[a.tile * D + 2 * rt] = M;
+          part[a.tile * D + 2 * rt + 1] = L;
         }
       }
     }

@@ -30,14 +30,48 @@ struct StoreArgs {
 
 constexpr int kHeld = 8;  // 16-byte vectors a thread keeps in registers
 
+// max |x| over a vector, as fp32; NaN is ignored (max returns its other operand), infinities are
+// not.  16-bit types compare in pairs.
+template <typename T, int VE>
+__device__ __forceinline__ float vec_amax(const ew::Vec<T, VE>& v) {
+  if constexpr (VE == 1 || sizeof(T) == 4) {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) m = fmaxf(m, fabsf(cvt<float>(v.v[e])));
+    return m;
+  } else {
+    using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const P* p = reinterpret_cast<const P*>(&v);
+    P m = __habs2(p[0]);
+#pragma unroll
+    for (int e = 1; e < VE / 2; ++e) m = __hmax2(m, __habs2(p[e]));
+    return fmaxf(cvt<float>(m.x), cvt<float>(m.y));
+  }
+}
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a <= 3.402823466e38f ? a : 0.f;  // infinities and NaN do not set the scale
 }
 
+// The vectors lane, lane + GT, ... of a page's rows: row and vector within the row, stepped
+// without a division.
+struct Walk {
+  int r, v, i;
+  __device__ __forceinline__ Walk(int lane, int vpr) : r(lane / vpr), v(lane - r * vpr), i(lane) {}
+  __device__ __forceinline__ void step(int n, int dr, int dv, int vpr) {
+    i += n;
+    r += dr;
+    v += dv;
+    if (v >= vpr) {
+      v -= vpr;
+      ++r;
+    }
+  }
+};
+
 // GT: threads of a group (32 or a whole block).  VEC: input rows and codes allow vectors.
 template <typename T, int CODE, int GT, bool VEC>
-__global__ void __launch_bounds__(GT == 32 ? 128 : GT) store_kernel(StoreArgs a) {
+__global__ void __launch_bounds__(GT == 32 ? 128 : GT, GT == 256 ? 4 : 8) store_kernel(StoreArgs a) {
   constexpr int VE = VEC ? 16 / (int)sizeof(T) : 1;
   constexpr int kThreads = GT == 32 ? 128 : GT;
   using V = ew::Vec<T, VE>;
@@ -45,11 +79,12 @@ __global__ void __launch_bounds__(GT == 32 ? 128 : GT) store_kernel(StoreArgs a)
   const int64_t unit = (int64_t)blockIdx.x * (kThreads / GT) + (GT == 32 ? threadIdx.x / 32 : 0);
   if (unit >= a.units) return;  // whole warps (GT 32) or no block (GT = block) leave here
   const int lane = GT == 32 ? threadIdx.x % 32 : threadIdx.x;
-  const int which = (int)(unit & 1);
-  int64_t u = unit >> 1;
-  const int j = (int)(u % a.cover);
-  u /= a.cover;
-  const int h = (int)(u % a.c.H), b = (int)(u / a.c.H);
+  // heads fastest: neighbouring groups read neighbouring rows of a [B, S, H, D] input
+  int64_t u = unit / a.c.H;
+  const int h = (int)(unit - u * a.c.H);
+  const int which = (int)(u & 1);
+  u >>= 1;
+  const int b = (int)(u / a.cover), j = (int)(u - (int64_t)b * a.cover);
   const int start = a.start[(int64_t)b * a.st_s];
   const int n = a.counts == nullptr ? a.S : min(max(a.counts[(int64_t)b * a.ct_s], 0), a.S);
   const int T_ = a.c.T, D = a.c.D;
@@ -58,55 +93,70 @@ __global__ void __launch_bounds__(GT == 32 ? 128 : GT) store_kernel(StoreArgs a)
   const int64_t p0 = (int64_t)m * T_;                 // position of the page's first token
   const int64_t lo = max((int64_t)start, p0), hi = min((int64_t)start + n, p0 + T_);
   if (lo >= hi) return;
-  const int page = page_of(a.table, a.c.P, b, m);
-  if (page < 0) return;
+  const int page = page_of(a.table, a.c.P, b, m);     // needed last: its load overlaps the data's
   const int kept = (int)(lo - p0);                    // tokens of this row already in the page
   const int rows = (int)(hi - lo);
-  const T* x = reinterpret_cast<const T*>(which ? a.value : a.key) + (int64_t)b * (which ? a.v_b : a.k_b) +
-               (int64_t)h * (which ? a.v_h : a.k_h) + (int64_t)(lo - start) * (which ? a.v_s : a.k_s);
   const int64_t x_s = which ? a.v_s : a.k_s, x_d = which ? a.v_d : a.k_d;
-  uint8_t* codes = (which ? a.c.value : a.c.key) + (int64_t)page * (which ? a.c.v_p : a.c.k_p) +
-                   (int64_t)h * (which ? a.c.v_h : a.c.k_h);
-  const int64_t c_t = which ? a.c.v_t : a.c.k_t;
-  float* sp = (which ? a.c.value_scale : a.c.key_scale) + (int64_t)page * (which ? a.c.vs_p : a.c.ks_p) +
-              (int64_t)h * (which ? a.c.vs_h : a.c.ks_h);
-  const float s_old = kept > 0 ? *sp : 0.f;
+  const T* x = reinterpret_cast<const T*>(which ? a.value : a.key) + (int64_t)b * (which ? a.v_b : a.k_b) +
+               (int64_t)h * (which ? a.v_h : a.k_h) + (int64_t)(lo - start) * x_s;
 
   const int vpr = D / VE;           // vectors of a row
   const int total = rows * vpr;
-  auto load = [&](int i) -> V {
-    const int r = i / vpr, d = (i - r * vpr) * VE;
-    if constexpr (VEC) return ew::load_cs(reinterpret_cast<const V*>(x + (int64_t)r * x_s + d));
+  const int dr = GT / vpr, dv = GT - dr * vpr;
+  auto load = [&](const Walk& w) -> V {
+    if constexpr (VEC) return ew::load_cs(reinterpret_cast<const V*>(x + (int64_t)w.r * x_s + w.v * VE));
     V v;
-    v.v[0] = x[(int64_t)r * x_s + (int64_t)d * x_d];
+    v.v[0] = x[(int64_t)w.r * x_s + (int64_t)w.v * x_d];
     return v;
   };
+  const Walk w0(lane, vpr);
   V held[kHeld];
+  Walk w = w0;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    if (w.i < total) held[k] = load(w);
+    w.step(GT, dr, dv, vpr);
+  }
   float amax = 0.f;
 #pragma unroll
   for (int k = 0; k < kHeld; ++k)
-    if (lane + k * GT < total) held[k] = load(lane + k * GT);
+    if (lane + k * GT < total) amax = fmaxf(amax, vec_amax<T, VE>(held[k]));
+  for (; w.i < total; w.step(GT, dr, dv, vpr)) amax = fmaxf(amax, vec_amax<T, VE>(load(w)));  // larger pages
+  auto reduce = [&](float v) {
 #pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (lane + k * GT < total)
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if constexpr (GT > 32) {
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+      __syncthreads();
 #pragma unroll
-      for (int e = 0; e < VE; ++e) amax = fmaxf(amax, finite_abs(cvt<float>(held[k].v[e])));
-  for (int i = lane + kHeld * GT; i < total; i += GT) {  // pages larger than the registers hold
-    const V v = load(i);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) amax = fmaxf(amax, finite_abs(cvt<float>(v.v[e])));
+      for (int q = 0; q < kThreads / 32; ++q) v = fmaxf(v, red[q]);
+    }
+    return v;
+  };
+  float* sp = nullptr;
+  uint8_t* codes = nullptr;
+  float s_old = 0.f;
+  const int64_t c_t = which ? a.c.v_t : a.c.k_t;
+  if (page >= 0) {
+    codes = (which ? a.c.value : a.c.key) + (int64_t)page * (which ? a.c.v_p : a.c.k_p) +
+            (int64_t)h * (which ? a.c.v_h : a.c.k_h);
+    sp = (which ? a.c.value_scale : a.c.key_scale) + (int64_t)page * (which ? a.c.vs_p : a.c.ks_p) +
+         (int64_t)h * (which ? a.c.vs_h : a.c.ks_h);
+    if (kept > 0) s_old = *sp;
   }
+  amax = reduce(amax);  // every thread of the group has read s_old by now
+  if (page < 0) return;
+  if (amax > 3.402823466e38f) {  // an infinity among the elements: once more without them
+    if constexpr (GT > 32) __syncthreads();
+    amax = 0.f;
+    for (Walk q = w0; q.i < total; q.step(GT, dr, dv, vpr)) {
+      const V v = load(q);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if constexpr (GT > 32) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, red[w]);
-  } else {
-    __syncwarp();
+      for (int e = 0; e < VE; ++e) amax = fmaxf(amax, finite_abs(cvt<float>(v.v[e])));
+    }
+    amax = reduce(amax);
   }
-  // every thread of the group has read s_old by now
+  if constexpr (GT == 32) __syncwarp();
   const float s_new = pow2(scale_exp<CODE>(amax));
   const float s = kept > 0 ? fmaxf(s_old, s_new) : s_new;
   if (lane == 0 && s != s_old) *sp = s;
@@ -118,25 +168,27 @@ __global__ void __launch_bounds__(GT == 32 ? 128 : GT) store_kernel(StoreArgs a)
     }
   }
   const float inv = 1.f / s;  // exact, as is every product with it: s is a power of two
-  auto put = [&](int i, const V& v) {
-    const int r = i / vpr, d = (i - r * vpr) * VE;
-    uint8_t* c = codes + (int64_t)(kept + r) * c_t + d;
+  auto put = [&](const Walk& q, const V& v) {
+    uint8_t* c = codes + (int64_t)(kept + q.r) * c_t + q.v * VE;
     if constexpr (VEC) {
-      uint32_t w[VE / 4];
+      uint32_t wd[VE / 4];
 #pragma unroll
       for (int e = 0; e < VE; e += 4)
-        w[e / 4] = encode4<CODE>(cvt<float>(v.v[e]) * inv, cvt<float>(v.v[e + 1]) * inv, cvt<float>(v.v[e + 2]) * inv,
-                                 cvt<float>(v.v[e + 3]) * inv);
-      if constexpr (VE == 8) *reinterpret_cast<uint2*>(c) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t*>(c) = w[0];
+        wd[e / 4] = encode4<CODE>(cvt<float>(v.v[e]) * inv, cvt<float>(v.v[e + 1]) * inv, cvt<float>(v.v[e + 2]) * inv,
+                                  cvt<float>(v.v[e + 3]) * inv);
+      if constexpr (VE == 8) *reinterpret_cast<uint2*>(c) = make_uint2(wd[0], wd[1]);
+      else *reinterpret_cast<uint32_t*>(c) = wd[0];
     } else {
       *c = encode1<CODE>(cvt<float>(v.v[0]) * inv);
     }
   };
+  w = w0;
 #pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (lane + k * GT < total) put(lane + k * GT, held[k]);
-  for (int i = lane + kHeld * GT; i < total; i += GT) put(i, load(i));
+  for (int k = 0; k < kHeld; ++k) {
+    if (w.i < total) put(w, held[k]);
+    w.step(GT, dr, dv, vpr);
+  }
+  for (; w.i < total; w.step(GT, dr, dv, vpr)) put(w, load(w));
 }
 
 template <typename T, int CODE, bool VEC>

@@ -33,18 +33,24 @@ constexpr int kThreads = 128;
 constexpr int kUnit = 128;            // keys of a unit: 32 a warp
 constexpr float kGrow = 6.f;          // rows rescale when their maximum grows by more (p <= 2^6)
 
-// Two codes of `w` (bytes 0, 1 or 2, 3) -> fp16 pair.
-template <int CODE, int HI>
-__device__ __forceinline__ uint32_t widen2(uint32_t w) {
+// Four codes -> two fp16 pairs (bytes 0, 1 and 2, 3).
+template <int CODE>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (CODE == NTB_F8E4M3) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(HI ? w >> 16 : w & 0xFFFFu), __NV_E4M3);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   } else {
     // w holds code + 128 in each byte: 0x6400 | u is the fp16 number 1024 + u
-    const uint32_t u = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
     const __half2 k = __floats2half2_rn(1152.f, 1152.f);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), k);
-    return *reinterpret_cast<const uint32_t*>(&r);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), k);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), k);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
   }
 }
 template <int CODE>
@@ -167,8 +173,8 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
     }
-    const uint8_t* kbase = a.c.key + (int64_t)pc.head * a.c.k_h + 16 * t;
-    const uint8_t* vbase = a.c.value + (int64_t)pc.head * a.c.v_h + 4 * VW * g;
+    const uint8_t* kbase = a.c.key + (int64_t)pc.head * a.c.k_h + (int64_t)g * a.c.k_t + 16 * t;
+    const uint8_t* vbase = a.c.value + (int64_t)pc.head * a.c.v_h + (int64_t)(2 * t) * a.c.v_t + 4 * VW * g;
     const float* ksb = a.c.key_scale + (int64_t)pc.head * a.c.ks_h;
     const float* vsb = a.c.value_scale + (int64_t)pc.head * a.c.vs_h;
 
@@ -188,44 +194,35 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
     auto load_k = [&](int u, const int (&id)[2]) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        ks[j] = id[j] < 0 ? 0.f : ksb[(int64_t)id[j] * a.c.ks_p];
-        vs_next[j] = id[j] < 0 ? 0.f : vsb[(int64_t)id[j] * a.c.vs_p];
-        const uint8_t* p = kbase + (int64_t)id[j] * a.c.k_p +
-                           (int64_t)(in_page(u * kUnit + warp * 32 + 16 * j) + g) * a.c.k_t;
+        const int page = max(id[j], 0);  // a hole reads page 0 and is masked
+        ks[j] = ksb[(int64_t)page * a.c.ks_p];
+        vs_next[j] = id[j] < 0 ? 0.f : vsb[(int64_t)page * a.c.vs_p];
+        const uint8_t* p = kbase + (int64_t)page * a.c.k_p +
+                           (int64_t)in_page(u * kUnit + warp * 32 + 16 * j) * a.c.k_t;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int h = 0; h < H64; ++h) {
-            if (id[j] >= 0) {
-              load_codes<4>(p + (int64_t)n * 8 * a.c.k_t + 64 * h, kr[2 * j + n][h]);
-            } else {
-#pragma unroll
-              for (int w = 0; w < 4; ++w) kr[2 * j + n][h][w] = 0u;
-            }
-          }
+          for (int h = 0; h < H64; ++h)
+            load_codes<4>(p + (int64_t)n * 8 * a.c.k_t + 64 * h, kr[2 * j + n][h]);
       }
     };
     auto load_v = [&](int u, const int (&id)[2]) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint8_t* p = vbase + (int64_t)id[j] * a.c.v_p +
-                           (int64_t)(in_page(u * kUnit + warp * 32 + 16 * j) + 2 * t) * a.c.v_t;
+        const uint8_t* p = vbase + (int64_t)max(id[j], 0) * a.c.v_p +
+                           (int64_t)in_page(u * kUnit + warp * 32 + 16 * j) * a.c.v_t;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (id[j] >= 0) {
-            load_codes<VW>(p + (int64_t)((k & 1) + 8 * (k >> 1)) * a.c.v_t, vr[j][k]);
-          } else {
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vr[j][k][w] = 0u;
-          }
-        }
+        for (int k = 0; k < 4; ++k) load_codes<VW>(p + (int64_t)((k & 1) + 8 * (k >> 1)) * a.c.v_t, vr[j][k]);
       }
     };
 
     int id[2], id_next[2];
+    auto any_key = [&](int u) { return u < pc.u1 && u * kUnit + warp * 32 < k_end; };
     load_ids(pc.u0, id);
-    load_k(pc.u0, id);
-    load_v(pc.u0, id);
+    if (any_key(pc.u0)) {
+      load_k(pc.u0, id);
+      load_v(pc.u0, id);
+    }
     load_ids(pc.u0 + 1, id_next);
     for (int u = pc.u0; u < pc.u1; ++u) {
       const int kw = u * kUnit + warp * 32;
@@ -239,16 +236,17 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
         for (int h = 0; h < H64; ++h)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const uint32_t c = bias<CODE>(kr[n][h][w]);
+            uint32_t b0, b1;
+            widen4<CODE>(bias<CODE>(kr[n][h][w]), b0, b1);
             mma_f16(s[n], qa[0][h * 4 + w][0], RT == 2 ? qa[RT - 1][h * 4 + w][0] : 0u, qa[0][h * 4 + w][1],
-                    RT == 2 ? qa[RT - 1][h * 4 + w][1] : 0u, widen2<CODE, 0>(c), widen2<CODE, 1>(c));
+                    RT == 2 ? qa[RT - 1][h * 4 + w][1] : 0u, b0, b1);
           }
       }
       const float ks_cur[2] = {ks[0], ks[1]};
       const bool hole[2] = {id[0] < 0, id[1] < 0};
       vs[0] = vs_next[0];
       vs[1] = vs_next[1];
-      load_k(u + 1, id_next);
+      if (any_key(u + 1)) load_k(u + 1, id_next);
       // ------------------------------------------------------------- softmax ----
       const bool edge = kw + 31 > k_low || hole[0] || hole[1];
       float alpha[RT];
@@ -314,13 +312,13 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
           pb[x][n >> 1][n & 1] = pack_f16(p0 * f, p1 * f);
         }
       }
-      // codes past the last key hold anything: 0 * NaN would not be 0
-      if (kw + 32 > k_end) {
+      // codes past the last key and in page 0 for a hole hold anything: 0 * NaN would not be 0
+      if (kw + 32 > k_end || hole[0] || hole[1]) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (kw + 16 * j + 2 * t + (k & 1) + 8 * (k >> 1) >= k_end)
+            if (hole[j] || kw + 16 * j + 2 * t + (k & 1) + 8 * (k >> 1) >= k_end)
 #pragma unroll
               for (int w = 0; w < VW; ++w) vr[j][k][w] = 0u;
       }
@@ -335,13 +333,14 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
           for (int i = 0; i < 2; ++i) {
             const uint32_t x01 = __byte_perm(v0, v1, i ? 0x7362 : 0x5140);
             const uint32_t x23 = __byte_perm(v2, v3, i ? 0x7362 : 0x5140);
-            const uint32_t a0 = widen2<CODE, 0>(x01), a1 = widen2<CODE, 1>(x01);
-            const uint32_t a2 = widen2<CODE, 0>(x23), a3 = widen2<CODE, 1>(x23);
+            uint32_t a0, a1, a2, a3;
+            widen4<CODE>(x01, a0, a1);
+            widen4<CODE>(x23, a2, a3);
 #pragma unroll
             for (int x = 0; x < RT; ++x) mma_f16(o[x][2 * w + i], a0, a1, a2, a3, pb[x][j][0], pb[x][j][1]);
           }
         }
-      load_v(u + 1, id_next);
+      if (any_key(u + 1)) load_v(u + 1, id_next);
       id[0] = id_next[0];
       id[1] = id_next[1];
       load_ids(u + 2, id_next);
@@ -432,7 +431,7 @@ bool decode_takes(const AttnArgs& a, int dtype) {
   auto al = [](const uint8_t* p, int64_t s0, int64_t s1, int64_t s2) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s0 % 16 == 0 && s1 % 16 == 0 && s2 % 16 == 0;
   };
-  return (dtype == NTB_BF16 || dtype == NTB_F16) && (c.D == 64 || c.D == 128) && c.T % 16 == 0 &&
+  return (dtype == NTB_BF16 || dtype == NTB_F16) && (c.D == 64 || c.D == 128) && c.T % 16 == 0 && c.P > 0 &&
          al(c.key, c.k_p, c.k_h, c.k_t) && al(c.value, c.v_p, c.v_h, c.v_t);
 }
 

@@ -60,7 +60,7 @@ __device__ __forceinline__ uint32_t bias(uint32_t w) {
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -230,18 +230,19 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
       // ------------------------------------------------------------- S = Q K^T ----
       float s[4][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      // keys innermost: four independent accumulators in turn
 #pragma unroll
-        for (int h = 0; h < H64; ++h)
+      for (int h = 0; h < H64; ++h)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
             uint32_t b0, b1;
             widen4<CODE>(bias<CODE>(kr[n][h][w]), b0, b1);
             mma_f16(s[n], qa[0][h * 4 + w][0], RT == 2 ? qa[RT - 1][h * 4 + w][0] : 0u, qa[0][h * 4 + w][1],
                     RT == 2 ? qa[RT - 1][h * 4 + w][1] : 0u, b0, b1);
           }
-      }
       const float ks_cur[2] = {ks[0], ks[1]};
       const bool hole[2] = {id[0] < 0, id[1] < 0};
       vs[0] = vs_next[0];

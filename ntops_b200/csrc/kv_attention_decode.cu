@@ -7,30 +7,37 @@
 // round to fp16 (2^-11).  ks_j multiplies scores, vs_j probabilities, relative to the largest
 // vs of the warp so far (O is rescaled when it grows, as when the row maximum does).
 //
-// Operands come straight from global memory into registers; neither product needs a byte moved
+// A producer warp copies units of 128 keys into a ring of shared-memory stages with TMA, one box
+// for the part of a page that a unit covers (up to 128 tokens of one page and head, whatever the
+// cache's strides), together with the pages' scales.  Four consumer warps take 32 keys each, as
+// four score tiles of 8 columns; column c of tile n is key 8n + row_of(c), chosen so that the
+// 16-byte loads below hit every bank once under TMA's swizzle.  Neither product needs a byte moved
 // between lanes, because a contraction may run over its index in any order:
-//   S = Q K^T: lane (g, t) loads 16 consecutive bytes of key 8n + g at channel 64h + 16t; bytes
+//   S = Q K^T: lane (g, t) loads 16 consecutive bytes of its key at channel 64h + 16t; bytes
 //     4s .. 4s + 3 are its B fragment of step (h, s), the query fragments are laid out alike;
-//   O^T = V^T P^T: lane (g, t) loads 16 channels at 16g of keys 2t, 2t + 1, 2t + 8, 2t + 9 of a
-//     16-key group; byte permutes pair two keys of one channel, and m-tile i takes channels
-//     16g + 2i (rows 0-7) and 16g + 2i + 1 (rows 8-15).  S's accumulators are P^T's B fragment.
-// With the queries as the 8 columns of O^T, up to 8 rows cost one product a group and 32
+//   O^T = V^T P^T: lane (g, t) loads 16 channels at 16g (D 128) of four keys; byte permutes pair two
+//     keys of one channel, and m-tile i takes channels 16g + 2i (rows 0-7) and 16g + 2i + 1 (rows
+//     8-15).  S's accumulators are P^T's B fragment.
+// With the queries as the 8 columns of O^T, up to 8 rows cost one product a group of 16 keys and 32
 // accumulators (RT = 1); 9 to 16 rows two (RT = 2).
 //
-// What bounds it: HBM.  A warp reads 32 keys (8 KB) at a time; the next 32 keys' loads are issued
-// as soon as the registers are free, page ids one block earlier still.
+// What bounds it: HBM.  Loading the codes straight into registers instead (no ring; 168 registers,
+// 12 warps an SM, ids and addresses computed by every warp) took 89 us on 32 rows of 4 to 8 k
+// tokens (8 kv heads of 128): twice the instructions, too few loads in flight.
 #include <algorithm>
 #include <type_traits>
 
 #include "kv_attention.cuh"
 #include "sm100.cuh"
+#include "tma.cuh"
 
 namespace ntb {
 namespace kv {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kUnit = 128;            // keys of a unit: 32 a warp
+constexpr int kConsumers = 4;
+constexpr int kThreads = 32 * (kConsumers + 1);
+constexpr int kUnit = 128;            // keys of a unit: 32 a consumer warp
 constexpr float kGrow = 6.f;          // rows rescale when their maximum grows by more (p <= 2^6)
 
 // Four codes -> two fp16 pairs (bytes 0, 1 and 2, 3).
@@ -70,40 +77,192 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Codes are read once: no L1 allocation.
-template <int W>
-__device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t (&r)[W]) {
-  if constexpr (W == 4)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "l"(p));
-  else
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
 }
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <int D, int RT>
-constexpr int min_blocks() {
-  return D == 128 ? (RT == 1 ? 3 : 2) : (RT == 1 ? 5 : 4);
+struct Cfg {
+  static constexpr int K_BYTES = kUnit * D, V_BYTES = kUnit * D;
+  static constexpr int STAGE = K_BYTES + V_BYTES;    // 1024-byte aligned for the swizzle
+  // Blocks an SM and stages a block: three blocks of two stages (64 KB each) where registers
+  // allow three blocks, else two of three.
+  static constexpr int BLOCKS = D == 128 ? (RT == 1 ? 3 : 2) : (RT == 1 ? 4 : 3);
+  static constexpr int STAGES = D == 128 ? (RT == 1 ? 2 : 3) : 3;
+  static constexpr int OS = D + 4;                   // padded row of the merge buffer (floats)
+  static constexpr int REC = STAGES * STAGE;         // {ks, vs, page id} of a stage's 8 groups of 16 keys
+  static constexpr int BUF = REC + STAGES * 128;     // float [8 RT][OS], then max, sum [8 RT]
+  static constexpr int BAR = BUF + 8 * RT * (OS + 2) * 4;
+  static constexpr int PRE = BAR + 16 * STAGES + 16;
+  static constexpr int SLACK = 1024;                 // to align the dynamic shared memory
+  static_assert(STAGE % 1024 == 0 && BAR % 16 == 0, "alignment");
+};
+
+// Row of column c in its group of 8 keys.  TMA's swizzle moves the 16-byte chunk x of row r to x ^
+// (r & 7) (128-byte rows) or x ^ ((r >> 1) & 3) (64-byte rows).  A K load's quarter warp reads four
+// chunks of columns 2q and 2q + 1: their rows must differ in bit 2 (in bit 0 for 64-byte rows,
+// two of which share the banks).  A V load's lanes read chunks of the even or of the odd columns:
+// their rows' bits 1 and 2 (64-byte rows: bit 0 and bit 2) must all differ.
+template <int D>
+__device__ __forceinline__ int row_of(int c) {
+  if constexpr (D == 128) return c ^ ((c & 1) << 2);                                // 0 5 2 7 4 1 6 3
+  return (((c >> 1) & 1) << 2) | ((c & 1) << 1) | (((c >> 2) ^ c) & 1);             // 0 3 4 7 1 2 5 6
+}
+template <int D>
+__device__ __forceinline__ uint32_t swizzled(int row, int byte) {  // offset of a byte of a row in a tile
+  if constexpr (D == 128) return row * 128 + (byte ^ ((row & 7) << 4));
+  return row * 64 + (byte ^ (((row >> 1) & 3) << 4));
+}
+
+// What the producer needs of a unit.
+struct Unit {
+  int b, head, key0, k_end;
+};
+
+// The end of the keys that any row of a tile sees.
+__device__ __forceinline__ int tile_end(const AttnArgs& a, int b, int tile, int rows_a_tile, int len, int start) {
+  return min(len, last_key(a, len, start, (min((tile + 1) * rows_a_tile, a.rows) - 1) / a.group) + 1);
 }
 
 template <typename T, int CODE, int D, int RT>
-__global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(AttnArgs a, int t_shift, int q_vec) {
+__global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
+    const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, AttnArgs a, int t_shift, int box,
+    int q_vec, int o_vec) {
+  using C = Cfg<D, RT>;
   constexpr int H64 = D / 64;       // 16-byte loads of a key row per lane
   constexpr int VW = D / 32;        // words of a lane's V channels: 4 (D 128) or 2 (D 64)
   constexpr int MT = D / 16;        // m-tiles of O^T
   constexpr int ROWS = 8 * RT;
-  constexpr int OS = D + 4;         // padded row of the merge buffer
-  extern __shared__ int pre[];
-  __shared__ __align__(16) float so[4][ROWS][OS];
-  __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
+  extern __shared__ __align__(128) uint8_t dyn_raw[];
+  uint8_t* dyn = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_raw) + 1023) & ~uintptr_t(1023));
+  float* buf = reinterpret_cast<float*>(dyn + C::BUF);
+  float* buf_m = buf + ROWS * C::OS;
+  float* buf_l = buf_m + ROWS;
+  uint64_t* full = reinterpret_cast<uint64_t*>(dyn + C::BAR);
+  uint64_t* empty = full + C::STAGES;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + C::STAGES);
+  int* pre = reinterpret_cast<int*>(dyn + C::PRE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      sm100::mbar_init(&full[s], 1);
+      sm100::mbar_init(&empty[s], kConsumers);
+    }
+    *abort_flag = 0;
+    sm100::fence_mbar_init();
+  }
   grid_dependency_launch();  // the joining kernel may start; it waits for this one before it reads
-  prefix_units<kThreads>(a, pre);
+  prefix_units<kThreads>(a, pre);  // (its barriers publish the mbarriers)
   const Line line(a, pre);
   if ((int)blockIdx.x >= line.blocks) return;
   const int64_t lo = line.begin(blockIdx.x), hi = line.begin(blockIdx.x + 1);
 
+  if (warp == kConsumers) {
+    // ----------------------------------------------------------------- producer ----
+    // lanes 0-7: the unit's 8 groups of 16 keys of K; lanes 8-15: of V.  The lane of a box's first
+    // group copies it.
+    const int grp = lane & 7;
+    const bool is_v = lane >= 8, first = lane < 16 && (16 * grp) % box == 0;
+    const float* scales = is_v ? a.c.value_scale : a.c.key_scale;
+    const int64_t s_p = is_v ? a.c.vs_p : a.c.ks_p, s_h = is_v ? a.c.vs_h : a.c.ks_h;
+    Piece pc;
+    int64_t pos = lo;
+    int u = 0, k_end = 0;
+    pc.u1 = 0;
+    // the next unit of this block's share; b = -1 past its end
+    auto advance = [&]() -> Unit {
+      if (u >= pc.u1) {
+        if (pos >= hi) return Unit{-1, 0, 0, 0};
+        pc = piece_at(a, line, pre, pos, lo, hi);
+        pos = pc.next;
+        u = pc.u0;
+        const int len = row_length(a, pc.b);
+        k_end = tile_end(a, pc.b, pc.tile, ROWS, len, row_start(a, pc.b, len));
+      }
+      return Unit{pc.b, pc.head, kUnit * u++, k_end};
+    };
+    auto page_id = [&](const Unit& w) {  // as the table has it
+      const int key = w.key0 + 16 * grp;
+      if (w.b < 0 || key >= w.k_end || lane >= 16) return -1;
+      const int m = t_shift >= 0 ? key >> t_shift : key / a.c.T;  // < M: lengths end with the table
+      return a.table.ids[(int64_t)w.b * a.table.s_b + (int64_t)m * a.table.s_m];
+    };
+    auto page_scale = [&](const Unit& w, int id) {
+      return id < 0 ? 0.f : scales[(int64_t)id * s_p + (int64_t)w.head * s_h];
+    };
+    auto checked = [&](int id) { return (unsigned)id < (unsigned)a.c.P ? id : -1; };
+    // Ids are loaded two units ahead, scales one: a load's result is not used before the next wait.
+    Unit w0 = advance();
+    int id0 = checked(page_id(w0));
+    Unit w1 = advance();
+    int id1 = page_id(w1);
+    float sc0 = page_scale(w0, id0);
+    int issued = 0;
+    for (; w0.b >= 0; ++issued) {
+      const int st = issued % C::STAGES;
+      int ok = 1;
+      if (lane == 0 && issued >= C::STAGES)
+        ok = sm100::mbar_wait(&empty[st], (uint32_t)((issued / C::STAGES - 1) & 1), abort_flag, a.err);
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      const bool mine = first && id0 >= 0;
+      const unsigned boxes = __ballot_sync(0xffffffffu, mine);
+      // The stage's one arrival comes after the scales are written; the copies' bytes are
+      // announced before the first can land.
+      if (lane == 0)
+        asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(sm100::smem_u32(&full[st])),
+                     "r"((uint32_t)__popc(boxes) * (uint32_t)(box * D))
+                     : "memory");
+      __syncwarp();
+      if (mine) {
+        const int key = w0.key0 + 16 * grp;
+        const int in_page = t_shift >= 0 ? key & (a.c.T - 1) : key % a.c.T;
+        sm100::tma_load_4d(dyn + st * C::STAGE + (is_v ? C::K_BYTES : 0) + 16 * grp * D, is_v ? &tv : &tk, &full[st], 0,
+                           in_page, w0.head, id0);
+      }
+      id1 = checked(id1);
+      if (lane < 16) {  // 16-byte records {ks, vs, id, -}
+        float* rec = reinterpret_cast<float*>(dyn + C::REC + st * 128) + grp * 4;
+        rec[is_v ? 1 : 0] = sc0;
+        if (!is_v) reinterpret_cast<int*>(rec)[2] = id0;
+      }
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&full[st]);
+      const Unit w2 = advance();
+      sc0 = page_scale(w1, id1);
+      w0 = w1;
+      id0 = id1;
+      w1 = w2;
+      id1 = page_id(w2);
+    }
+    // every copy has landed before the block's shared memory goes
+    if (lane == 0)
+      for (int i = max(issued - C::STAGES, 0); i < issued; ++i)
+        sm100::mbar_wait_unwind(&full[i % C::STAGES], (uint32_t)((i / C::STAGES) & 1));
+    return;
+  }
+
+  // --------------------------------------------------------------------- consumers ----
+  const int g = lane >> 2, t = lane & 3;
+  // This lane's K row (column g of tile 0), V rows (columns 2t and 2t + 1) in the warp's 32 keys;
+  // tile n's rows are 8n further on, which the swizzle does not see.
+  const uint32_t base = sm100::smem_u32(dyn) + warp * 32 * D;
+  const int kc[2] = {row_of<D>(2 * t), row_of<D>(2 * t + 1)};  // keys of columns 2t and 2t + 1 within a tile
+  uint32_t k_off[H64];
+#pragma unroll
+  for (int h = 0; h < H64; ++h) k_off[h] = base + swizzled<D>(row_of<D>(g), 64 * h + 16 * t);
+  const uint32_t v_off[2] = {base + C::K_BYTES + swizzled<D>(kc[0], 4 * VW * g),
+                             base + C::K_BYTES + swizzled<D>(kc[1], 4 * VW * g)};
+  const uint32_t rec_off = sm100::smem_u32(dyn) + C::REC + 32 * warp;
+  int it = 0;
+  bool ok = true;
   for (int64_t pos = lo; pos < hi;) {
     const Piece pc = piece_at(a, line, pre, pos, lo, hi);
     pos = pc.next;
@@ -162,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
     }
     // every row of the tile sees the keys up to k_low; none sees a key at or past k_end
     const int k_low = last_key(a, len, start, r0 / a.group);
-    const int k_end = min(len, last_key(a, len, start, (min(r0 + ROWS, a.rows) - 1) / a.group) + 1);
+    const int k_end = tile_end(a, pc.b, pc.tile, ROWS, len, start);
 
     float m[RT], l[RT], vref = 1.17549435e-38f, inv_vref = 1.f / vref;
     float o[RT][MT][4];
@@ -173,232 +332,254 @@ __global__ void __launch_bounds__(kThreads, min_blocks<D, RT>()) decode_kernel(A
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
     }
-    const uint8_t* kbase = a.c.key + (int64_t)pc.head * a.c.k_h + (int64_t)g * a.c.k_t + 16 * t;
-    const uint8_t* vbase = a.c.value + (int64_t)pc.head * a.c.v_h + (int64_t)(2 * t) * a.c.v_t + 4 * VW * g;
-    const float* ksb = a.c.key_scale + (int64_t)pc.head * a.c.ks_h;
-    const float* vsb = a.c.value_scale + (int64_t)pc.head * a.c.vs_h;
-
-    // ---------------------------------------------------- loads of one block of 32 keys ----
-    auto load_ids = [&](int u, int (&id)[2]) {
+    for (int u = pc.u0; u < pc.u1; ++u, ++it) {
+      const int st = it % C::STAGES;
+      if (ok) ok = sm100::mbar_wait(&full[st], (uint32_t)((it / C::STAGES) & 1), abort_flag, a.err);
+      if (!ok) break;
+      const int kw = u * kUnit + 32 * warp;  // column c of tile n is key kw + 8n + row_of(c)
+      if (kw < k_end) {
+        const uint4 rec0 = lds16(rec_off + st * 128), rec1 = lds16(rec_off + st * 128 + 16);
+        const float ks[2] = {__uint_as_float(rec0.x), __uint_as_float(rec1.x)};
+        const float vs[2] = {__uint_as_float(rec0.y), __uint_as_float(rec1.y)};
+        const bool hole[2] = {(int)rec0.z < 0, (int)rec1.z < 0};  // or a group past the last key
+        // ----------------------------------------------------------- S = Q K^T ----
+        float s[4][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int key = u * kUnit + warp * 32 + 16 * j;
-        id[j] = -1;
-        if (u < pc.u1 && key < k_end)
-          id[j] = page_of(a.table, a.c.P, pc.b, t_shift >= 0 ? key >> t_shift : key / a.c.T);
-      }
-    };
-    auto in_page = [&](int key) { return t_shift >= 0 ? key & (a.c.T - 1) : key % a.c.T; };
-    uint32_t kr[4][H64][4], vr[2][4][VW];
-    float ks[2], vs[2], vs_next[2];
-    auto load_k = [&](int u, const int (&id)[2]) {
+        for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        // keys innermost: four independent accumulators in turn
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int page = max(id[j], 0);  // a hole reads page 0 and is masked
-        ks[j] = ksb[(int64_t)page * a.c.ks_p];
-        vs_next[j] = id[j] < 0 ? 0.f : vsb[(int64_t)page * a.c.vs_p];
-        const uint8_t* p = kbase + (int64_t)page * a.c.k_p +
-                           (int64_t)in_page(u * kUnit + warp * 32 + 16 * j) * a.c.k_t;
+        for (int h = 0; h < H64; ++h) {
+          uint4 kr[4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < 4; ++n) kr[n] = lds16(k_off[h] + st * C::STAGE + 8 * n * D);
 #pragma unroll
-          for (int h = 0; h < H64; ++h)
-            load_codes<4>(p + (int64_t)n * 8 * a.c.k_t + 64 * h, kr[2 * j + n][h]);
-      }
-    };
-    auto load_v = [&](int u, const int (&id)[2]) {
+          for (int w = 0; w < 4; ++w)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint8_t* p = vbase + (int64_t)max(id[j], 0) * a.c.v_p +
-                           (int64_t)in_page(u * kUnit + warp * 32 + 16 * j) * a.c.v_t;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) load_codes<VW>(p + (int64_t)((k & 1) + 8 * (k >> 1)) * a.c.v_t, vr[j][k]);
-      }
-    };
-
-    int id[2], id_next[2];
-    auto any_key = [&](int u) { return u < pc.u1 && u * kUnit + warp * 32 < k_end; };
-    load_ids(pc.u0, id);
-    if (any_key(pc.u0)) {
-      load_k(pc.u0, id);
-      load_v(pc.u0, id);
-    }
-    load_ids(pc.u0 + 1, id_next);
-    for (int u = pc.u0; u < pc.u1; ++u) {
-      const int kw = u * kUnit + warp * 32;
-      if (kw >= k_end) break;  // (later blocks too)
-      // ------------------------------------------------------------- S = Q K^T ----
-      float s[4][4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      // keys innermost: four independent accumulators in turn
-#pragma unroll
-      for (int h = 0; h < H64; ++h)
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            uint32_t b0, b1;
-            widen4<CODE>(bias<CODE>(kr[n][h][w]), b0, b1);
-            mma_f16(s[n], qa[0][h * 4 + w][0], RT == 2 ? qa[RT - 1][h * 4 + w][0] : 0u, qa[0][h * 4 + w][1],
-                    RT == 2 ? qa[RT - 1][h * 4 + w][1] : 0u, b0, b1);
-          }
-      const float ks_cur[2] = {ks[0], ks[1]};
-      const bool hole[2] = {id[0] < 0, id[1] < 0};
-      vs[0] = vs_next[0];
-      vs[1] = vs_next[1];
-      if (any_key(u + 1)) load_k(u + 1, id_next);
-      // ------------------------------------------------------------- softmax ----
-      const bool edge = kw + 31 > k_low || hole[0] || hole[1];
-      float alpha[RT];
-      bool grown = false;
-#pragma unroll
-      for (int x = 0; x < RT; ++x) {
-        float mb = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float sc = rowsc[x] * ks_cur[n >> 1];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float v = s[n][2 * x + e] * sc;
-            if (edge) {
-              const int key = kw + 8 * n + 2 * t + e;
-              if (key > kmax[x] || hole[n >> 1]) v = -INFINITY;
+            for (int n = 0; n < 4; ++n) {
+              const uint32_t c = w == 0 ? kr[n].x : w == 1 ? kr[n].y : w == 2 ? kr[n].z : kr[n].w;
+              uint32_t b0, b1;
+              widen4<CODE>(bias<CODE>(c), b0, b1);
+              mma_f16(s[n], qa[0][h * 4 + w][0], RT == 2 ? qa[RT - 1][h * 4 + w][0] : 0u, qa[0][h * 4 + w][1],
+                      RT == 2 ? qa[RT - 1][h * 4 + w][1] : 0u, b0, b1);
             }
-            s[n][2 * x + e] = v;
-            mb = fmaxf(mb, v);
-          }
         }
-        mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
-        mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
-        alpha[x] = 1.f;
-        if (mb > m[x] + kGrow) {
-          alpha[x] = exp2f(m[x] - mb);  // 0 at the first block that the row sees
-          m[x] = mb;
-          grown = true;
-        }
-      }
-      float vmul = 1.f;
-      const float vtop = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
-      if (vtop > vref) {  // the same for every lane
-        vmul = vref / vtop;
-        vref = vtop;
-        inv_vref = 1.f / vtop;
-      }
-      if (__any_sync(0xffffffffu, grown) || vmul != 1.f) {
+        // ------------------------------------------------------------- softmax ----
+        const bool edge = kw + 31 > k_low || hole[0] || hole[1];  // the same for every lane
+        float alpha[RT];
+        bool grown = false;
 #pragma unroll
         for (int x = 0; x < RT; ++x) {
-          l[x] *= alpha[x];
-          // O^T's columns are rows 2t and 2t + 1, whose statistics lanes 8t and 8t + 4 hold
-          const float a0 = __shfl_sync(0xffffffffu, alpha[x], 8 * t) * vmul;
-          const float a1 = __shfl_sync(0xffffffffu, alpha[x], 8 * t + 4) * vmul;
+          float mb = -INFINITY;
+          const float sc[2] = {rowsc[x] * ks[0], rowsc[x] * ks[1]};
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            o[x][i][0] *= a0;
-            o[x][i][1] *= a1;
-            o[x][i][2] *= a0;
-            o[x][i][3] *= a1;
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v = s[n][2 * x + e] * sc[n >> 1];
+              if (edge && (hole[n >> 1] || kw + 8 * n + kc[e] > kmax[x])) v = -INFINITY;
+              s[n][2 * x + e] = v;
+              mb = fmaxf(mb, v);
+            }
+          mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+          mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
+          alpha[x] = 1.f;
+          if (mb > m[x] + kGrow) {
+            alpha[x] = exp2f(m[x] - mb);  // 0 at the first block that the row sees
+            m[x] = mb;
+            grown = true;
+          }
+        }
+        const float vtop = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
+        float vmul = 1.f;
+        if (vtop > vref) {  // the same for every lane
+          vmul = vref / vtop;
+          vref = vtop;
+          inv_vref = 1.f / vtop;
+        }
+        if (__any_sync(0xffffffffu, grown) || vmul != 1.f) {
+#pragma unroll
+          for (int x = 0; x < RT; ++x) {
+            l[x] *= alpha[x];
+            // O^T's columns are rows 2t and 2t + 1, whose statistics lanes 8t and 8t + 4 hold
+            const float a0 = __shfl_sync(0xffffffffu, alpha[x], 8 * t) * vmul;
+            const float a1 = __shfl_sync(0xffffffffu, alpha[x], 8 * t + 4) * vmul;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              o[x][i][0] *= a0;
+              o[x][i][1] *= a1;
+              o[x][i][2] *= a0;
+              o[x][i][3] *= a1;
+            }
+          }
+        }
+        uint32_t pb[RT][2][2];
+        const float f[2] = {vs[0] * inv_vref, vs[1] * inv_vref};
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+          const float ref = m[x] == -INFINITY ? 0.f : m[x];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float p0 = sm100::ex2_approx(s[n][2 * x] - ref), p1 = sm100::ex2_approx(s[n][2 * x + 1] - ref);
+            l[x] += p0 + p1;
+            pb[x][n >> 1][n & 1] = pack_f16(p0 * f[n >> 1], p1 * f[n >> 1]);
+          }
+        }
+        // ------------------------------------------------------- O^T += V^T P^T ----
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t vr[4][VW];  // keys (column 2t, tile 2j), (2t + 1, 2j), (2t, 2j + 1), (2t + 1, 2j + 1)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t at = v_off[k & 1] + st * C::STAGE + 8 * (2 * j + (k >> 1)) * D;
+            if constexpr (VW == 4) {
+              const uint4 x = lds16(at);
+              vr[k][0] = x.x; vr[k][1] = x.y; vr[k][VW - 2] = x.z; vr[k][VW - 1] = x.w;
+            } else {
+              const uint2 x = lds8(at);
+              vr[k][0] = x.x; vr[k][1] = x.y;
+            }
+          }
+          // what lies past the last key or in a hole's place is anything: 0 * NaN would not be 0
+          if (edge) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (hole[j] || kw + 8 * (2 * j + (k >> 1)) + kc[k & 1] >= k_end)
+#pragma unroll
+                for (int w = 0; w < VW; ++w) vr[k][w] = 0u;
+          }
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            const uint32_t v0 = bias<CODE>(vr[0][w]), v1 = bias<CODE>(vr[1][w]);
+            const uint32_t v2 = bias<CODE>(vr[2][w]), v3 = bias<CODE>(vr[3][w]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t x01 = __byte_perm(v0, v1, i ? 0x7362 : 0x5140);
+              const uint32_t x23 = __byte_perm(v2, v3, i ? 0x7362 : 0x5140);
+              uint32_t a0, a1, a2, a3;
+              widen4<CODE>(x01, a0, a1);
+              widen4<CODE>(x23, a2, a3);
+#pragma unroll
+              for (int x = 0; x < RT; ++x) mma_f16(o[x][2 * w + i], a0, a1, a2, a3, pb[x][j][0], pb[x][j][1]);
+            }
           }
         }
       }
-      uint32_t pb[RT][2][2];
-#pragma unroll
-      for (int x = 0; x < RT; ++x) {
-        const float ref = m[x] == -INFINITY ? 0.f : m[x];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float p0 = sm100::ex2_approx(s[n][2 * x] - ref), p1 = sm100::ex2_approx(s[n][2 * x + 1] - ref);
-          l[x] += p0 + p1;
-          const float f = vs[n >> 1] * inv_vref;
-          pb[x][n >> 1][n & 1] = pack_f16(p0 * f, p1 * f);
-        }
-      }
-      // codes past the last key and in page 0 for a hole hold anything: 0 * NaN would not be 0
-      if (kw + 32 > k_end || hole[0] || hole[1]) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (hole[j] || kw + 16 * j + 2 * t + (k & 1) + 8 * (k >> 1) >= k_end)
-#pragma unroll
-              for (int w = 0; w < VW; ++w) vr[j][k][w] = 0u;
-      }
-      // ------------------------------------------------------------- O^T += V^T P^T ----
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          const uint32_t v0 = bias<CODE>(vr[j][0][w]), v1 = bias<CODE>(vr[j][1][w]);
-          const uint32_t v2 = bias<CODE>(vr[j][2][w]), v3 = bias<CODE>(vr[j][3][w]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t x01 = __byte_perm(v0, v1, i ? 0x7362 : 0x5140);
-            const uint32_t x23 = __byte_perm(v2, v3, i ? 0x7362 : 0x5140);
-            uint32_t a0, a1, a2, a3;
-            widen4<CODE>(x01, a0, a1);
-            widen4<CODE>(x23, a2, a3);
-#pragma unroll
-            for (int x = 0; x < RT; ++x) mma_f16(o[x][2 * w + i], a0, a1, a2, a3, pb[x][j][0], pb[x][j][1]);
-          }
-        }
-      if (any_key(u + 1)) load_v(u + 1, id_next);
-      id[0] = id_next[0];
-      id[1] = id_next[1];
-      load_ids(u + 2, id_next);
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&empty[st]);  // this warp is done with the stage
     }
-    // --------------------------------------------------- join the four warps' results ----
+    // --------------------------------------------- join the warps' results, 3 -> 2 -> 1 -> 0 ----
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      if (t == 0) {
-        sm_m[warp][8 * x + g] = m[x];
-        sm_l[warp][8 * x + g] = l[x];
-      }
-      // channels 4 VW g + 2i (elements 0, 1) and + 2i + 1 (2, 3) of rows 2t and 2t + 1
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int i = 0; i < MT; i += 2)
-          *reinterpret_cast<float4*>(&so[warp][8 * x + 2 * t + e][4 * VW * g + 2 * i]) =
-              make_float4(o[x][i][e] * vref, o[x][i][2 + e] * vref, o[x][i + 1][e] * vref, o[x][i + 1][2 + e] * vref);
+        for (int e = 0; e < 4; ++e) o[x][i][e] *= vref;
     }
-    __syncthreads();
-    const int rows = min(ROWS, a.rows - r0);
-    for (int idx = threadIdx.x; idx < rows * D; idx += kThreads) {
-      const int rt = idx / D, d = idx % D, r = r0 + rt;
-      float M = sm_m[0][rt];
+#pragma unroll 1
+    for (int w = kConsumers - 1; w > 0; --w) {
+      if (warp == w) {
 #pragma unroll
-      for (int w = 1; w < 4; ++w) M = fmaxf(M, sm_m[w][rt]);
-      const float ref = M == -INFINITY ? 0.f : M;
-      float L = 0.f, acc = 0.f;
+        for (int x = 0; x < RT; ++x) {
+          if (t == 0) {
+            buf_m[8 * x + g] = m[x];
+            buf_l[8 * x + g] = l[x];
+          }
+          // channels 4 VW g + 2i (elements 0, 1) and + 2i + 1 (2, 3) of rows 2t and 2t + 1
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = exp2f(sm_m[w][rt] - ref);
-        L = fmaf(sm_l[w][rt], f, L);
-        acc = fmaf(so[w][rt][d], f, acc);
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < MT; i += 2)
+              *reinterpret_cast<float4*>(&buf[(8 * x + 2 * t + e) * C::OS + 4 * VW * g + 2 * i]) =
+                  make_float4(o[x][i][e], o[x][i][2 + e], o[x][i + 1][e], o[x][i + 1][2 + e]);
+        }
       }
-      if (pc.whole) {
-        reinterpret_cast<T*>(a.o)[(int64_t)pc.b * a.o_b + (int64_t)(pc.head * a.group + r % a.group) * a.o_h +
-                                  (int64_t)(r / a.group) * a.o_s + d] = cvt<T>(L == 0.f ? 0.f : acc / L);
-      } else {
-        float* part = a.part + (int64_t)pc.slot * slot_floats(a.tile, D);
-        part[rt * D + d] = acc;
-        if (d == 0) {
-          part[a.tile * D + 2 * rt] = M;
-          part[a.tile * D + 2 * rt + 1] = L;
+      consumer_sync();
+      if (warp == w - 1) {
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+          const float mo = buf_m[8 * x + g], M = fmaxf(m[x], mo), ref = M == -INFINITY ? 0.f : M;
+          const float fa = exp2f(m[x] - ref), fb = exp2f(mo - ref);
+          l[x] = l[x] * fa + buf_l[8 * x + g] * fb;
+          m[x] = M;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float a0 = __shfl_sync(0xffffffffu, fa, 8 * t + 4 * e), b0 = __shfl_sync(0xffffffffu, fb, 8 * t + 4 * e);
+#pragma unroll
+            for (int i = 0; i < MT; i += 2) {
+              const float4 y = *reinterpret_cast<const float4*>(&buf[(8 * x + 2 * t + e) * C::OS + 4 * VW * g + 2 * i]);
+              o[x][i][e] = fmaf(o[x][i][e], a0, y.x * b0);
+              o[x][i][2 + e] = fmaf(o[x][i][2 + e], a0, y.y * b0);
+              o[x][i + 1][e] = fmaf(o[x][i + 1][e], a0, y.z * b0);
+              o[x][i + 1][2 + e] = fmaf(o[x][i + 1][2 + e], a0, y.w * b0);
+            }
+          }
+        }
+        __syncwarp();  // it may write the buffer next
+      }
+    }
+    consumer_sync();  // warp 0 has read the buffer before the next piece writes it
+    if (warp == 0 && ok) {
+#pragma unroll
+      for (int x = 0; x < RT; ++x) {
+        const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int rt = 8 * x + 2 * t + e, r = r0 + rt;
+          const float iv = __shfl_sync(0xffffffffu, inv, 8 * t + 4 * e);
+          const float L = __shfl_sync(0xffffffffu, l[x], 8 * t + 4 * e);
+          if (r >= a.rows) continue;
+          if (pc.whole) {
+            T* op = reinterpret_cast<T*>(a.o) + (int64_t)pc.b * a.o_b +
+                    (int64_t)(pc.head * a.group + r % a.group) * a.o_h + (int64_t)(r / a.group) * a.o_s + 4 * VW * g;
+            ew::Vec<T, 2 * MT> y;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              y.v[2 * i] = cvt<T>(L == 0.f ? 0.f : o[x][i][e] * iv);
+              y.v[2 * i + 1] = cvt<T>(L == 0.f ? 0.f : o[x][i][2 + e] * iv);
+            }
+            if (o_vec) {
+#pragma unroll
+              for (int i = 0; i < 2 * MT; i += 8)
+                *reinterpret_cast<uint4*>(op + i) = *reinterpret_cast<const uint4*>(&y.v[i]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2 * MT; ++i) op[i] = y.v[i];
+            }
+          } else {
+            float* part = a.part + (int64_t)pc.slot * slot_floats(a.tile, D) + rt * D + 4 * VW * g;
+#pragma unroll
+            for (int i = 0; i < MT; i += 2)
+              *reinterpret_cast<float4*>(part + 2 * i) =
+                  make_float4(o[x][i][e], o[x][i][2 + e], o[x][i + 1][e], o[x][i + 1][2 + e]);
+          }
+        }
+        if (!pc.whole && t == 0) {
+          float* part = a.part + (int64_t)pc.slot * slot_floats(a.tile, D) + (int64_t)a.tile * D + 2 * (8 * x + g);
+          part[0] = m[x];
+          part[1] = l[x];
         }
       }
     }
-    __syncthreads();  // before the next piece writes the merge buffers
   }
+}
+
+// Map of a layer's codes (D, T, H, P), swizzled over a row of D bytes.  A size-1 dimension is never
+// stepped, so it takes any stride that TMA accepts.
+int code_map(CUtensorMap* map, uint8_t* base, const Layer& c, int64_t s_t, int64_t s_h, int64_t s_p, int box) {
+  return tma::encode_4d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, c.D, c.T, c.H, c.P, c.T > 1 ? s_t : 16,
+                        c.H > 1 ? s_h : 16, c.P > 1 ? s_p : 16, c.D, box,
+                        c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 template <typename T, int CODE, int D, int RT>
 int go(const AttnArgs& a, cudaStream_t st, int* blocks) {
   auto k = decode_kernel<T, CODE, D, RT>;
-  if (blocks != nullptr) {  // asked for a full batch's unit counts, whatever this launch's batch
-    *blocks = resident_blocks((const void*)k, kThreads, sizeof(int) * (a.nb + 1));
+  const size_t smem = Cfg<D, RT>::SLACK + Cfg<D, RT>::PRE + sizeof(int) * (a.nb + 1);
+  NTB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+  if (blocks != nullptr) {
+    *blocks = resident_blocks((const void*)k, kThreads, smem);
     return NTB_OK;
   }
   const bool pow2_page = (a.c.T & (a.c.T - 1)) == 0;
@@ -406,7 +587,15 @@ int go(const AttnArgs& a, cudaStream_t st, int* blocks) {
   while (pow2_page && (1 << shift) < a.c.T) ++shift;
   const int q_vec = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && (a.q_b % 8 == 0 || a.table.B == 1) &&
                     (a.q_h % 8 == 0 || a.Hq == 1) && (a.q_s % 8 == 0 || a.Sq == 1);
-  k<<<a.G, kThreads, sizeof(int) * (a.nb + 1), st>>>(a, pow2_page ? shift : -1, q_vec);
+  const int o_vec = reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && (a.o_b % 8 == 0 || a.table.B == 1) &&
+                    (a.o_h % 8 == 0 || a.Hq == 1) && (a.o_s % 8 == 0 || a.Sq == 1);
+  int box = 16;  // tokens of a TMA box: the largest power of two up to a unit that divides a page
+  while (box < kUnit && a.c.T % (2 * box) == 0) box *= 2;
+  CUtensorMap tk, tv;
+  int rc;
+  if ((rc = code_map(&tk, a.c.key, a.c, a.c.k_t, a.c.k_h, a.c.k_p, box)) != NTB_OK) return rc;
+  if ((rc = code_map(&tv, a.c.value, a.c, a.c.v_t, a.c.v_h, a.c.v_p, box)) != NTB_OK) return rc;
+  k<<<a.G, kThreads, smem, st>>>(tk, tv, a, pow2_page ? shift : -1, box, q_vec, o_vec);
   NTB_LAUNCH_CHECK();
   return NTB_OK;
 }
@@ -426,11 +615,12 @@ int go_any(const AttnArgs& a, int dtype, cudaStream_t st, int* blocks) {
 
 }  // namespace
 
-// 16-bit queries, head_dim 64 or 128, pages that hold whole 16-key groups, 16-byte rows.
+// 16-bit queries, head_dim 64 or 128, pages of whole 16-key groups, strides that TMA takes.
 bool decode_takes(const AttnArgs& a, int dtype) {
   const Layer& c = a.c;
-  auto al = [](const uint8_t* p, int64_t s0, int64_t s1, int64_t s2) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s0 % 16 == 0 && s1 % 16 == 0 && s2 % 16 == 0;
+  auto al = [&](const uint8_t* p, int64_t s_p, int64_t s_h, int64_t s_t) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (c.P == 1 || tma::stride_ok(s_p)) &&
+           (c.H == 1 || tma::stride_ok(s_h)) && (c.T == 1 || tma::stride_ok(s_t));
   };
   return (dtype == NTB_BF16 || dtype == NTB_F16) && (c.D == 64 || c.D == 128) && c.T % 16 == 0 && c.P > 0 &&
          al(c.key, c.k_p, c.k_h, c.k_t) && al(c.value, c.v_p, c.v_h, c.v_t);

@@ -6,6 +6,7 @@ to the sm_100a kernels of the shared library on the caller's current CUDA stream
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -88,18 +89,23 @@ class NtbTensor(ctypes.Structure):
     ]
 
 
-class NtbKvCache(ctypes.Structure):
-    _fields_ = [
-        ("key", NtbTensor),
-        ("value", NtbTensor),
-        ("key_scale", NtbTensor),
-        ("value_scale", NtbTensor),
-    ]
-
-
 _P = ctypes.POINTER(NtbTensor)
-_PC = ctypes.POINTER(NtbKvCache)
+_PB = ctypes.c_char_p  # a descriptor as packed bytes (pack_desc), read by the call only
 _VP = ctypes.c_void_p
+
+# NtbTensor layouts by rank: pointer, dtype, ndim, the sizes, the strides (each padded to MAX_DIMS).
+_PACK = tuple(
+    struct.Struct(f"Pii{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x").pack if n else struct.Struct("Pii128x").pack
+    for n in range(MAX_DIMS + 1)
+)
+
+
+def pack_desc(t, code):
+    """The bytes of t's NtbTensor with the given dtype code: a quarter of the time that filling the
+    ctypes structure takes, for calls whose kernels last a few microseconds.  No checks."""
+    n = t.dim()
+    return _PACK[n](t.data_ptr(), code, n, *t.shape, *t.stride())
+
 _SIGNATURES = {
     "ntb_version": ([], ctypes.c_int),
     "ntb_last_error": ([], ctypes.c_char_p),
@@ -134,16 +140,16 @@ _SIGNATURES = {
         ctypes.c_int,
     ),
     "ntb_sdpa_decode_static": ([_P, _P, _P, _P, _P, ctypes.c_double, ctypes.c_int, _VP], ctypes.c_int),
-    "ntb_kv_store": ([_PC, _P, _P, _P, _P, _P, _VP], ctypes.c_int),
-    "ntb_kv_attention_workspace": ([_P, _PC, _P, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
+    "ntb_kv_store": ([_PB, _PB, _PB, _PB, _PB, _PB, _VP], ctypes.c_int),
+    "ntb_kv_attention_workspace": ([_PB, _PB, _PB, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
     "ntb_kv_attention": (
-        [_P, _PC, _P, _P, _P, _P, ctypes.c_double, ctypes.c_int, _VP, ctypes.c_int64, _VP],
+        [_PB, _PB, _PB, _PB, _PB, _PB, ctypes.c_double, ctypes.c_int, _VP, ctypes.c_int64, _VP],
         ctypes.c_int,
     ),
-    "ntb_kv_copy_pages": ([_PC, _P, _P, _VP], ctypes.c_int),
-    "ntb_kv_extend": ([_P, _P, _P, ctypes.c_int64, _P, _P, _P, _VP, ctypes.c_int64, _VP], ctypes.c_int),
-    "ntb_kv_reorder": ([_PC, _P, _P, _P, _P, _P, _P, _P, _P, _VP, ctypes.c_int64, _VP], ctypes.c_int),
-    "ntb_kv_compact": ([_PC, _P, _P, _P, _P, _P, _VP, ctypes.c_int64, _VP], ctypes.c_int),
+    "ntb_kv_copy_pages": ([_PB, _PB, _PB, _VP], ctypes.c_int),
+    "ntb_kv_extend": ([_PB, _PB, _PB, ctypes.c_int64, _PB, _PB, _PB, _VP, ctypes.c_int64, _VP], ctypes.c_int),
+    "ntb_kv_reorder": ([_PB, _PB, _PB, _PB, _PB, _PB, _PB, _PB, _PB, _VP, ctypes.c_int64, _VP], ctypes.c_int),
+    "ntb_kv_compact": ([_PB, _PB, _PB, _PB, _PB, _PB, _VP, ctypes.c_int64, _VP], ctypes.c_int),
 }
 
 _lib = None

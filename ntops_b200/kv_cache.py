@@ -26,32 +26,42 @@ import math
 import torch
 
 from ntops_b200 import _lib
-from ntops_b200.torch.utils import _check_cuda, launch, lib
+from ntops_b200.torch import utils as _utils
+from ntops_b200.torch.utils import _check_cuda, lib
 
 _CODES = {torch.float8_e4m3fn: 10, torch.int8: _lib.DTYPE_CODES[torch.int8]}
-_QUERY_TYPES = (torch.bfloat16, torch.float16, torch.float32)
-_DIMS = ctypes.c_int64 * _lib.MAX_DIMS
+_QUERY_TYPES = {t: _lib.DTYPE_CODES[t] for t in (torch.bfloat16, torch.float16, torch.float32)}
+_F32 = _lib.DTYPE_CODES[torch.float32]
+_I32 = _lib.DTYPE_CODES[torch.int32]
+_INT = {torch.int32: _I32}
+_pack = _lib.pack_desc
 
 
-def _desc(t, code):
-    return _lib.NtbTensor(t.data_ptr(), code, t.dim(), _DIMS(*t.shape), _DIMS(*t.stride()))
-
-
-def _tensor(t, name, device, dtypes, ndim):
-    """Descriptor of an operand after the checks that need Python's view of it."""
+def _tensor(t, name, device, codes, ndim):
+    """Packed descriptor of an operand after the checks that need Python's view of it."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if t.device != device:
         _check_cuda(t)
         raise RuntimeError(f"{name} is on {t.device}, the cache on {device}")
-    if t.dtype not in dtypes:
-        raise RuntimeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    code = codes.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{name} must be one of {', '.join(str(d) for d in codes)}, got {t.dtype}")
     if t.dim() != ndim:
         raise RuntimeError(f"{name} must be {ndim}-D, got {t.dim()}-D")
-    return _desc(t, _lib.DTYPE_CODES[t.dtype])
+    return _pack(t, code)
 
 
-_I32 = (torch.int32,)
+def _call(what, fn, index, *args):
+    """fn(*args, stream) on the current stream of device `index`, with that device current."""
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, what)
+    _utils.launch_count += 1
 
 
 class _CacheView:
@@ -60,10 +70,10 @@ class _CacheView:
     def __init__(self, key, value, key_scale, value_scale):
         self.key, self.value, self.key_scale, self.value_scale = key, value, key_scale, value_scale
         self.device = key.device
-        self._c = _lib.NtbKvCache(_desc(key, _CODES[key.dtype]), _desc(value, _CODES[value.dtype]),
-                                  _desc(key_scale, _lib.DTYPE_CODES[torch.float32]),
-                                  _desc(value_scale, _lib.DTYPE_CODES[torch.float32]))
-        self._ref = ctypes.byref(self._c)
+        self._index = key.device.index
+        code = _CODES[key.dtype]
+        self._desc = _pack(key, code) + _pack(value, code) + _pack(key_scale, _F32) + _pack(value_scale, _F32)
+        self._workspace = {}  # attention: bytes of workspace by the sizes that decide them
 
 
 class PagedKVLayer(_CacheView):
@@ -143,10 +153,10 @@ def store(layer, key, value, block_table, start, counts=None):
     c = _view(layer, PagedKVLayer, "store")
     kd = _tensor(key, "key", c.device, _QUERY_TYPES, 4)
     vd = _tensor(value, "value", c.device, _QUERY_TYPES, 4)
-    td = _tensor(block_table, "block_table", c.device, _I32, 2)
-    sd = _tensor(start, "start", c.device, _I32, 1)
-    nd = None if counts is None else _tensor(counts, "counts", c.device, _I32, 1)
-    launch("kv_store", lib().ntb_kv_store, c._ref, kd, vd, td, sd, nd, device_tensor=c.key)
+    td = _tensor(block_table, "block_table", c.device, _INT, 2)
+    sd = _tensor(start, "start", c.device, _INT, 1)
+    nd = None if counts is None else _tensor(counts, "counts", c.device, _INT, 1)
+    _call("kv_store", lib().ntb_kv_store, c._index, c._desc, kd, vd, td, sd, nd)
 
 
 def attention(query, layer, block_table, lengths, scale=None, is_causal=True, start=None):
@@ -159,21 +169,25 @@ def attention(query, layer, block_table, lengths, scale=None, is_causal=True, st
     default.  A query that sees no key gives zeros.  Softmax statistics and sums are in fp32."""
     c = _view(layer, PagedKVLayer, "attention")
     qd = _tensor(query, "query", c.device, _QUERY_TYPES, 4)
-    td = _tensor(block_table, "block_table", c.device, _I32, 2)
-    ld = _tensor(lengths, "lengths", c.device, _I32, 1)
-    sd = None if start is None else _tensor(start, "start", c.device, _I32, 1)
+    td = _tensor(block_table, "block_table", c.device, _INT, 2)
+    ld = _tensor(lengths, "lengths", c.device, _INT, 1)
+    sd = None if start is None else _tensor(start, "start", c.device, _INT, 1)
     if query.shape[-1] > 1 and query.stride(-1) != 1:
         raise RuntimeError("query must have a unit inner stride")
     if scale is None:
         scale = 1 / math.sqrt(query.shape[-1])
     L = lib()
-    nbytes = ctypes.c_int64(0)
-    with _lib.device_of(query):
-        _lib.check(L.ntb_kv_attention_workspace(qd, c._ref, td, ctypes.byref(nbytes)), "kv_attention")
+    sizes = (query.shape, query.dtype, block_table.shape[1])
+    nbytes = c._workspace.get(sizes)
+    if nbytes is None:
+        n = ctypes.c_int64(0)
+        with torch.cuda.device(c._index):
+            _lib.check(L.ntb_kv_attention_workspace(qd, c._desc, td, ctypes.byref(n)), "kv_attention")
+        nbytes = c._workspace[sizes] = n.value
     output = torch.empty_like(query)
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=c.device)
-    launch("kv_attention", L.ntb_kv_attention, qd, c._ref, td, ld, sd, _desc(output, qd.dtype), float(scale),
-           int(bool(is_causal)), ctypes.c_void_p(ws.data_ptr()), nbytes.value, device_tensor=output)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=c.device)
+    _call("kv_attention", L.ntb_kv_attention, c._index, qd, c._desc, td, ld, sd, _pack(output, _QUERY_TYPES[query.dtype]),
+          scale, bool(is_causal), ws.data_ptr(), nbytes)
     return output
 
 
@@ -181,12 +195,12 @@ def copy_pages(cache, src, dst):
     """Copies pages src[k] to dst[k] (int32 [n]) with their scales, in every layer.  No page may be
     both a source and a destination, nor twice a destination; pairs out of range are skipped."""
     c = _view(cache, PagedKVCache, "copy_pages")
-    sd, dd = _tensor(src, "src", c.device, _I32, 1), _tensor(dst, "dst", c.device, _I32, 1)
-    launch("kv_copy_pages", lib().ntb_kv_copy_pages, c._ref, sd, dd, device_tensor=c.key)
+    sd, dd = _tensor(src, "src", c.device, _INT, 1), _tensor(dst, "dst", c.device, _INT, 1)
+    _call("kv_copy_pages", lib().ntb_kv_copy_pages, c._index, c._desc, sd, dd)
 
 
 def _refs(refs, c):
-    d = _tensor(refs, "refs", c.device, _I32, 1)
+    d = _tensor(refs, "refs", c.device, _INT, 1)
     if refs.shape[0] != c.num_pages:
         raise RuntimeError(f"refs has {refs.shape[0]} entries, the cache {c.num_pages} pages")
     if not refs.is_contiguous():
@@ -199,13 +213,13 @@ def extend(cache, block_table, refs, lengths):
     lowest-numbered free page, in row order.  Returns ``(block_table, refs, missing)``, new tensors;
     missing, int32 [1], counts entries that found no free page and stay holes."""
     c = _view(cache, PagedKVCache, "extend")
-    td, rd = _tensor(block_table, "block_table", c.device, _I32, 2), _refs(refs, c)
-    ld = _tensor(lengths, "lengths", c.device, _I32, 1)
+    td, rd = _tensor(block_table, "block_table", c.device, _INT, 2), _refs(refs, c)
+    ld = _tensor(lengths, "lengths", c.device, _INT, 1)
     table = torch.empty(block_table.shape, dtype=torch.int32, device=c.device)
     out, missing = torch.empty_like(refs), torch.empty(1, dtype=torch.int32, device=c.device)
     ws = torch.empty(max(block_table.numel(), 1), dtype=torch.int32, device=c.device)
-    launch("kv_extend", lib().ntb_kv_extend, td, ld, rd, c.page_size, _desc(table, td.dtype), _desc(out, td.dtype),
-           _desc(missing, td.dtype), ctypes.c_void_p(ws.data_ptr()), 4 * ws.numel(), device_tensor=c.key)
+    _call("kv_extend", lib().ntb_kv_extend, c._index, td, ld, rd, c.page_size, _pack(table, _I32), _pack(out, _I32),
+          _pack(missing, _I32), ws.data_ptr(), 4 * ws.numel())
     return table, out, missing
 
 
@@ -220,16 +234,15 @@ def reorder(cache, block_table, lengths, refs, parents):
     ``(block_table [N, M], lengths [N], refs, missing)``, new tensors; missing, int32 [1], counts
     copies that found no free page (their entries are holes: take pages back before going on)."""
     c = _view(cache, PagedKVCache, "reorder")
-    td, rd = _tensor(block_table, "block_table", c.device, _I32, 2), _refs(refs, c)
-    ld, pd = _tensor(lengths, "lengths", c.device, _I32, 1), _tensor(parents, "parents", c.device, _I32, 1)
+    td, rd = _tensor(block_table, "block_table", c.device, _INT, 2), _refs(refs, c)
+    ld, pd = _tensor(lengths, "lengths", c.device, _INT, 1), _tensor(parents, "parents", c.device, _INT, 1)
     n = parents.shape[0]
     table = torch.empty((n, block_table.shape[1]), dtype=torch.int32, device=c.device)
     lens, out = torch.empty(n, dtype=torch.int32, device=c.device), torch.empty_like(refs)
     missing = torch.empty(1, dtype=torch.int32, device=c.device)
     ws = torch.empty(4 * n + 1, dtype=torch.int32, device=c.device)
-    i32 = td.dtype
-    launch("kv_reorder", lib().ntb_kv_reorder, c._ref, td, ld, rd, pd, _desc(table, i32), _desc(lens, i32),
-           _desc(out, i32), _desc(missing, i32), ctypes.c_void_p(ws.data_ptr()), 4 * ws.numel(), device_tensor=c.key)
+    _call("kv_reorder", lib().ntb_kv_reorder, c._index, c._desc, td, ld, rd, pd, _pack(table, _I32), _pack(lens, _I32),
+          _pack(out, _I32), _pack(missing, _I32), ws.data_ptr(), 4 * ws.numel())
     return table, lens, out, missing
 
 
@@ -238,11 +251,10 @@ def compact(cache, block_table, refs):
     the k-th used page past the first U moves to the k-th free page among them.  Returns
     ``(block_table, refs, used)``, new tensors; used, int32 [1], is U: pages from U on are free."""
     c = _view(cache, PagedKVCache, "compact")
-    td, rd = _tensor(block_table, "block_table", c.device, _I32, 2), _refs(refs, c)
+    td, rd = _tensor(block_table, "block_table", c.device, _INT, 2), _refs(refs, c)
     table = torch.empty(block_table.shape, dtype=torch.int32, device=c.device)
     out, used = torch.empty_like(refs), torch.empty(1, dtype=torch.int32, device=c.device)
     ws = torch.empty(3 * c.num_pages + 1, dtype=torch.int32, device=c.device)
-    i32 = td.dtype
-    launch("kv_compact", lib().ntb_kv_compact, c._ref, td, rd, _desc(table, i32), _desc(out, i32), _desc(used, i32),
-           ctypes.c_void_p(ws.data_ptr()), 4 * ws.numel(), device_tensor=c.key)
+    _call("kv_compact", lib().ntb_kv_compact, c._index, c._desc, td, rd, _pack(table, _I32), _pack(out, _I32),
+          _pack(used, _I32), ws.data_ptr(), 4 * ws.numel())
     return table, out, used

@@ -5,8 +5,8 @@
 // past the query's position start[b] + i; zero where no key is left.  ks_j and vs_j are the
 // scales of token j's page, which multiply scores and probabilities instead of 2 * D values.
 //
-// kv_attention_decode.cu holds the tensor-core kernel for few rows.  This file has the entry
-// points, the kernel for every other case (fp32 queries, any head_dim up to 256, any page size:
+// kv_attention_decode.cu holds the tensor-core kernel for up to 16 packed rows (query heads of a
+// group times queries), kv_attention_sm100.cu the one for more.  This file has the entry points, the kernel for every other case (fp32 queries, any head_dim up to 256, any page size:
 // CUDA-core dot products over 32-key tiles staged in fp32) and the kernel that joins the partial
 // results of segments cut over the key range.
 #include <algorithm>
@@ -319,11 +319,22 @@ int fill(const NtbTensor* q, const NtbKvCache* cache, const NtbTensor* table, At
   return NTB_OK;
 }
 
+// The kernel that takes a call.
+enum class Path { generic, decode, prompt };
+Path path_of(const AttnArgs& a, int dtype) {
+  if (!tensor_cores_take(a, dtype)) return Path::generic;
+  return a.rows <= 16 ? Path::decode : Path::prompt;
+}
+
 // Tile, unit and number of blocks for a launch of up to kMaxBatch batch rows.
 int plan(AttnArgs* a, int dtype) {
   a->b0 = 0;
   a->nb = std::min(a->table.B, kMaxBatch);
-  if (decode_takes(*a, dtype)) return decode_plan(a, dtype);
+  switch (path_of(*a, dtype)) {
+    case Path::decode: return decode_plan(a, dtype);
+    case Path::prompt: prompt_plan(a); return NTB_OK;
+    default: break;
+  }
   a->tile = kGenTile;
   a->unit = kGenUnit;
   a->tiles = (a->rows + a->tile - 1) / a->tile;
@@ -333,6 +344,17 @@ int plan(AttnArgs* a, int dtype) {
 int64_t part_bytes(const AttnArgs& a) { return 2ll * a.G * slot_floats(a.tile, a.c.D) * (int64_t)sizeof(float); }
 
 }  // namespace
+
+bool tensor_cores_take(const AttnArgs& a, int dtype) {
+  const Layer& c = a.c;
+  auto al = [&](const uint8_t* p, int64_t s_p, int64_t s_h, int64_t s_t) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (c.P == 1 || tma::stride_ok(s_p)) &&
+           (c.H == 1 || tma::stride_ok(s_h)) && (c.T == 1 || tma::stride_ok(s_t));
+  };
+  return (dtype == NTB_BF16 || dtype == NTB_F16) && (c.D == 64 || c.D == 128) && c.T % 16 == 0 && c.P > 0 &&
+         al(c.key, c.k_p, c.k_h, c.k_t) && al(c.value, c.v_p, c.v_h, c.v_t);
+}
+
 }  // namespace kv
 }  // namespace ntb
 
@@ -377,16 +399,24 @@ extern "C" int ntb_kv_attention(const NtbTensor* q, const NtbKvCache* cache, con
   a.scale = (float)scale;
   a.causal = causal != 0;
   if ((rc = plan(&a, q->dtype)) != NTB_OK) return rc;
-  NTB_ARG(workspace != nullptr && workspace_bytes >= part_bytes(a), "workspace too small: %lld bytes, need %lld",
+  NTB_ARG((workspace != nullptr || part_bytes(a) == 0) && workspace_bytes >= part_bytes(a), "workspace too small: %lld bytes, need %lld",
           (long long)workspace_bytes, (long long)part_bytes(a));
   NTB_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
   a.part = reinterpret_cast<float*>(workspace);
   cudaStream_t st = (cudaStream_t)stream;
   for (a.b0 = 0; a.b0 < a.table.B; a.b0 += kMaxBatch) {
     a.nb = std::min(a.table.B - a.b0, kMaxBatch);
-    rc = decode_takes(a, q->dtype) ? decode_launch(a, q->dtype, st) : generic_any(a, q->dtype, st, nullptr);
+    switch (path_of(a, q->dtype)) {
+      case Path::prompt: rc = prompt_launch(a, q->dtype, st); break;
+      case Path::decode:
+        rc = decode_launch(a, q->dtype, st);
+        if (rc == NTB_OK) rc = combine_launch(a, q->dtype, st);
+        break;
+      default:
+        rc = generic_any(a, q->dtype, st, nullptr);
+        if (rc == NTB_OK) rc = combine_launch(a, q->dtype, st);
+    }
     if (rc != NTB_OK) return rc;
-    if ((rc = combine_launch(a, q->dtype, st)) != NTB_OK) return rc;
   }
   return NTB_OK;
 }

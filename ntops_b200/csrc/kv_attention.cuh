@@ -14,6 +14,7 @@
 #pragma once
 
 #include "kv_cache.cuh"
+#include "tma.cuh"
 
 namespace ntb {
 namespace kv {
@@ -137,10 +138,23 @@ __device__ __forceinline__ int last_key(const AttnArgs& a, int len, int start, i
   return p < 0 ? -1 : (int)min(p, (int64_t)len - 1);
 }
 
-// Launchers of the kernels; they fill tile / unit / G, and take `part` from the workspace.
-bool decode_takes(const AttnArgs& a, int dtype);
+// Map of a layer's codes (D, T, H, P) with the swizzle of D-byte rows, box of `box` tokens.  A size-1
+// dimension is never stepped, so it takes any stride that TMA accepts.
+inline int code_map(CUtensorMap* map, uint8_t* base, const Layer& c, int64_t s_t, int64_t s_h, int64_t s_p, int box) {
+  return tma::encode_4d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, c.D, c.T, c.H, c.P, c.T > 1 ? s_t : 16,
+                        c.H > 1 ? s_h : 16, c.P > 1 ? s_p : 16, c.D, box,
+                        c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+// Whether the tensor-core kernels take these operands (16-bit queries, head_dim 64 or 128, pages of
+// whole 16-key groups, strides that TMA accepts).
+bool tensor_cores_take(const AttnArgs& a, int dtype);
+// Up to 16 packed rows (kv_attention_decode.cu): plan fills tile, tiles, unit and G.
 int decode_plan(AttnArgs* a, int dtype);
 int decode_launch(const AttnArgs& a, int dtype, cudaStream_t st);
+// More rows (kv_attention_sm100.cu); joins its own pieces.
+void prompt_plan(AttnArgs* a);
+int prompt_launch(const AttnArgs& a, int dtype, cudaStream_t st);
 
 }  // namespace kv
 }  // namespace ntb

@@ -29,7 +29,6 @@
 
 #include "kv_attention.cuh"
 #include "sm100.cuh"
-#include "tma.cuh"
 
 namespace ntb {
 namespace kv {
@@ -565,14 +564,6 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
   }
 }
 
-// Map of a layer's codes (D, T, H, P), swizzled over a row of D bytes.  A size-1 dimension is never
-// stepped, so it takes any stride that TMA accepts.
-int code_map(CUtensorMap* map, uint8_t* base, const Layer& c, int64_t s_t, int64_t s_h, int64_t s_p, int box) {
-  return tma::encode_4d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, c.D, c.T, c.H, c.P, c.T > 1 ? s_t : 16,
-                        c.H > 1 ? s_h : 16, c.P > 1 ? s_p : 16, c.D, box,
-                        c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
-}
-
 template <typename T, int CODE, int D, int RT>
 int go(const AttnArgs& a, cudaStream_t st, int* blocks) {
   auto k = decode_kernel<T, CODE, D, RT>;
@@ -614,17 +605,6 @@ int go_any(const AttnArgs& a, int dtype, cudaStream_t st, int* blocks) {
 }
 
 }  // namespace
-
-// 16-bit queries, head_dim 64 or 128, pages of whole 16-key groups, strides that TMA takes.
-bool decode_takes(const AttnArgs& a, int dtype) {
-  const Layer& c = a.c;
-  auto al = [&](const uint8_t* p, int64_t s_p, int64_t s_h, int64_t s_t) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (c.P == 1 || tma::stride_ok(s_p)) &&
-           (c.H == 1 || tma::stride_ok(s_h)) && (c.T == 1 || tma::stride_ok(s_t));
-  };
-  return (dtype == NTB_BF16 || dtype == NTB_F16) && (c.D == 64 || c.D == 128) && c.T % 16 == 0 && c.P > 0 &&
-         al(c.key, c.k_p, c.k_h, c.k_t) && al(c.value, c.v_p, c.v_h, c.v_t);
-}
 
 int decode_plan(AttnArgs* a, int dtype) {
   a->tile = a->rows <= 8 ? 8 : 16;

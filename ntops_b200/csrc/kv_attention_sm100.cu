@@ -1,0 +1,774 @@
+// Attention of many query rows (prompts, chunks of them, long speculative blocks) over the paged
+// 8-bit KV cache, on tcgen05 tensor cores.
+//
+// A block owns two tiles of 128 packed rows (row = query * group + head of the group: one key
+// block serves the whole group) and walks its keys in blocks of 128:
+//   warp 1      looks up pages and scales and copies the codes of half a block (64 keys) of K or V
+//               at a time into staging slots with TMA;
+//   warps 4-7   widen codes to fp16 (exact) into the swizzled operand tiles, two of K and two of V;
+//   warp 0      issues S_t = Q_t K^T (both from shared memory) and O_t += P_t V (P from TMEM) in the
+//               order PV_0(j), S_0(j+1), PV_1(j), S_1(j+1): one tile's products run during the
+//               other's softmax;
+//   warps 8-15  one thread a row: load Q (multiplied by a power of two that puts the row's largest
+//               element in [2^14, 2^15), so fp16 holds it as exactly as the input type), take S from
+//               TMEM, keep the running maximum, write P = exp2(.) in fp16 over S.
+// Page scales: within a block keys are widened relative to the block's largest ks, values relative
+// to the largest vs so far (ratios are powers of two for what ntb_kv_store writes, so nothing
+// rounds outside fp16's subnormals); softmax multiplies scores by the block's ks, and O is rescaled
+// when vs grows, as when the row maximum does (only past 2^8, as P <= 2^8 fits fp16).
+//
+// What bounds it: the exponentials (2 x 128 x 128 of them a block on a 16-per-clock unit: 2048
+// cycles, the products' time as well).  Where one wave of blocks would leave SMs idle, several
+// blocks share a tile's keys and kv_split_combine joins them.
+#include <algorithm>
+#include <atomic>
+
+#include "kv_attention.cuh"
+#include "sm100.cuh"
+#include "tma.cuh"
+
+namespace ntb {
+namespace kv {
+namespace {
+
+constexpr int BLK = 128;
+constexpr int kTiles = 2;
+constexpr int kThreads = 512;
+constexpr int kMmaWarp = 0, kTmaWarp = 1, kConvBase = 4, kSoftBase = 8;
+// Register split (setmaxnreg) of 512 threads launched with 128 each: the sum over the warpgroups
+// must not exceed the launch's, or the raise would wait forever; the host checks the latter.
+constexpr int kLaunchRegs = 128, kProdRegs = 72, kConvRegs = 72, kSoftRegs = 184;
+static_assert(kProdRegs + kConvRegs + 2 * kSoftRegs <= 4 * kLaunchRegs, "register split too large");
+constexpr float kRescaleThreshold = 8.f;
+constexpr int kHalf = 64;       // keys of a staging slot
+constexpr int kInfo = 4;        // blocks whose scales are kept: see info_full below
+constexpr uint32_t kSCol = 0, kOCol = 256;  // TMEM columns: S_t at 128 t (P_t over its first 64), O_t at 256 + 128 t
+
+template <int D>
+struct Smem {
+  static constexpr int SUB = BLK * 128;          // [128 rows][64 fp16], 128-byte swizzle
+  static constexpr int NSUB = D / 64;
+  static constexpr int TILE = SUB * NSUB;
+  static constexpr int SLOT = kHalf * D;         // staged codes
+  static constexpr int Q = 0;                    // 2 tiles
+  static constexpr int K = Q + kTiles * TILE;    // 2 stages
+  static constexpr int V = K + 2 * TILE;
+  static constexpr int SK = V + 2 * TILE;        // 2 slots: the halves of a block
+  static constexpr int SV = SK + 2 * SLOT;
+  static constexpr int INFO = SV + 2 * SLOT;     // kInfo x 80 bytes
+  static constexpr int BAR = INFO + 512;
+  static constexpr int TOTAL = BAR + 256 + 1024;
+  static_assert(TOTAL <= 227 * 1024, "shared memory");
+};
+
+// Scales of a block: ratios of its 8 groups of 16 keys, then the block's.
+struct Info {
+  float kr[8], vr[8];
+  float kref;    // scores carry the ks / kref of their keys
+  float vfac;    // O's factor before this block: the previous vref over this one's
+  float vref;
+  uint32_t holes;  // bit g: group g has no page (or no key)
+};
+static_assert(sizeof(Info) * kInfo <= 512, "info ring");
+
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Four codes -> two fp16 pairs.
+template <int CODE>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CODE == NTB_F8E4M3) {
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  } else {
+    w ^= 0x80808080u;  // 0x6400 | u is the fp16 number 1024 + u
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 k = __floats2half2_rn(1152.f, 1152.f);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), k);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), k);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, __half2 f) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), f);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Row of lane group i (0-7) in 8 keys: two neighbouring groups' rows differ so that 16-byte loads of
+// the staged codes and stores of the fp16 tile hit every bank once under their swizzles.
+template <int D>
+__device__ __forceinline__ int row_of(int i) {
+  if constexpr (D == 128) return i ^ ((i & 1) << 2);
+  return (((i >> 1) & 1) << 2) | ((i & 1) << 1) | (((i >> 2) ^ i) & 1);
+}
+
+struct SplitArgs {
+  int splits;   // blocks that share a segment's keys
+  int box;      // tokens of a TMA box
+  int t_shift;  // log2 of the page size, or -1
+  int q_vec, o_vec;
+};
+
+// The segment of a block: heavy (late) row tiles of all batch rows and heads first.
+struct Where {
+  int b, head, tile, split;
+};
+__device__ __forceinline__ Where where_is(const AttnArgs& a, int splits, int64_t idx) {
+  Where w;
+  w.split = (int)(idx % splits);
+  idx /= splits;
+  w.head = (int)(idx % a.c.H);
+  idx /= a.c.H;
+  w.b = a.b0 + (int)(idx % a.nb);
+  w.tile = a.tiles - 1 - (int)(idx / a.nb);
+  return w;
+}
+
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, AttnArgs a,
+                  SplitArgs sa) {
+  using S = Smem<D>;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::BAR);
+  uint64_t* q_full = bars + 0;
+  uint64_t* k_full = bars + 1;    // [2] fp16 tiles
+  uint64_t* k_empty = bars + 3;   // [2]
+  uint64_t* v_full = bars + 5;    // [2]
+  uint64_t* v_empty = bars + 7;   // [2]
+  uint64_t* sk_full = bars + 9;   // [2] staged halves
+  uint64_t* sk_empty = bars + 11; // [2]
+  uint64_t* sv_full = bars + 13;  // [2]
+  uint64_t* sv_empty = bars + 15; // [2]
+  uint64_t* s_full = bars + 17;   // [tile]
+  uint64_t* p_full = bars + 19;   // [tile]
+  uint64_t* pv_done = bars + 21;  // [tile]
+  // [kInfo] scales of block j.  The producer writes entry j once K(j - 2)'s slots are free, that is
+  // after S_1(j - 3) was issued, which follows both tiles' P(j - 4): entry j - 4 is no longer read.
+  uint64_t* info_full = bars + 23;
+  uint64_t* done_bar = bars + 27;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  Info* info = reinterpret_cast<Info*>(sm + S::INFO);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Where w = where_is(a, sa.splits, blockIdx.x);
+  const int len = row_length(a, w.b), start = row_start(a, w.b, len);
+  const int r0 = w.tile * kTiles * BLK;
+  // Key blocks [jb, jb + n) of this block; tile t takes the first n_t of them.
+  int n_t[kTiles], k_end = 0, all = 0;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    n_t[t] = 0;
+    const int first = r0 + t * BLK, last = min(first + BLK, a.rows) - 1;
+    if (first < a.rows) {
+      const int e = min(len, last_key(a, len, start, last / a.group) + 1);
+      n_t[t] = (max(e, 0) + BLK - 1) / BLK;
+      k_end = max(k_end, e);
+      all = max(all, n_t[t]);
+    }
+  }
+  const int jb = (int)((int64_t)all * w.split / sa.splits), je = (int)((int64_t)all * (w.split + 1) / sa.splits);
+  int n = 0;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    n_t[t] = max(min(n_t[t], je) - jb, 0);
+    n = max(n, n_t[t]);
+  }
+
+  if (threadIdx.x == 0) {
+    sm100::mbar_init(q_full, 256);
+    for (int i = 0; i < 2; ++i) {
+      sm100::mbar_init(&k_full[i], 128);
+      sm100::mbar_init(&k_empty[i], 1);
+      sm100::mbar_init(&v_full[i], 128);
+      sm100::mbar_init(&v_empty[i], 1);
+      sm100::mbar_init(&sk_full[i], 1);
+      sm100::mbar_init(&sk_empty[i], 4);
+      sm100::mbar_init(&sv_full[i], 1);
+      sm100::mbar_init(&sv_empty[i], 4);
+      sm100::mbar_init(&s_full[i], 1);
+      sm100::mbar_init(&p_full[i], 128);
+      sm100::mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < kInfo; ++i) sm100::mbar_init(&info_full[i], 1);
+    sm100::mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    sm100::fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    sm100::tmem_alloc(tmem_slot, 512);
+    sm100::tmem_relinquish();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_launch();
+
+  if (warp < kConvBase) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProdRegs));
+    if (warp == kTmaWarp) {
+      // --------------------------------------------------------------- producer ----
+      // lanes 0-7: the block's 8 groups of 16 keys of K; lanes 8-15: of V.  The lane of a box's
+      // first group copies it.
+      const int grp = lane & 7;
+      const bool is_v = lane >= 8, mine = lane < 16;
+      const bool first = mine && (16 * grp) % sa.box == 0;
+      const float* scales = (is_v ? a.c.value_scale : a.c.key_scale) + (int64_t)w.head * (is_v ? a.c.vs_h : a.c.ks_h);
+      const int64_t s_p = is_v ? a.c.vs_p : a.c.ks_p;
+      const int* ids = a.table.ids + (int64_t)w.b * a.table.s_b;
+      auto page_id = [&](int j) {  // as the table has it
+        const int key = (jb + j) * BLK + 16 * grp;
+        if (!mine || j >= n || key >= k_end) return -1;
+        return ids[(int64_t)(sa.t_shift >= 0 ? key >> sa.t_shift : key / a.c.T) * a.table.s_m];
+      };
+      auto checked = [&](int id) { return (unsigned)id < (unsigned)a.c.P ? id : -1; };
+      auto page_scale = [&](int id) { return id < 0 ? 0.f : scales[(int64_t)id * s_p]; };
+      // Ids are loaded two blocks ahead, scales one.
+      int id0 = checked(page_id(0)), id1 = page_id(1);
+      float sc0 = page_scale(id0), vrun = 1.17549435e-38f;
+      bool ok = true;
+      int staged = 0;  // slots armed so far, in the order K0 K1 V0 V1 of each block
+      for (int j = 0; j < n && ok; ++j) {
+        id1 = checked(id1);
+        const float sc1 = page_scale(id1);
+        const int id2 = page_id(j + 2);
+        // the block's reference scales, over lanes 0-7 and 8-15
+        float top = mine ? fabsf(sc0) : 0.f;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float kref = fmaxf(__shfl_sync(0xffffffffu, top, 0), 1.17549435e-38f);
+        const float vold = vrun;
+        vrun = fmaxf(vrun, __shfl_sync(0xffffffffu, top, 8));
+        const uint32_t holes = ~__ballot_sync(0xffffffffu, id0 >= 0) & 0xFFu;
+        Info* I = &info[j % kInfo];
+        bool wrote = false;
+        for (int q = 0; q < 4 && ok; ++q) {
+          const int h = q & 1;
+          const bool v = q >= 2;
+          uint64_t* full = v ? &sv_full[h] : &sk_full[h];
+          uint64_t* empty = v ? &sv_empty[h] : &sk_empty[h];
+          int go = 1;
+          if (lane == 0) go = sm100::mbar_wait(empty, (uint32_t)((j & 1) ^ 1), abort_flag, a.err);
+          ok = __shfl_sync(0xffffffffu, go, 0);
+          if (!ok) break;
+          if (!wrote) {  // K's slots are free: so is the entry
+            if (mine) (is_v ? I->vr : I->kr)[grp] = sc0 / (is_v ? vrun : kref);
+            if (lane == 0) {
+              I->kref = kref;
+              I->vfac = j == 0 ? 1.f : vold / vrun;
+              I->vref = vrun;
+              I->holes = holes;
+            }
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&info_full[j % kInfo]);
+            wrote = true;
+          }
+          const bool go_mine = first && is_v == v && (grp >> 2) == h && id0 >= 0;
+          const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, go_mine));
+          if (lane == 0) sm100::mbar_arrive_expect_tx(full, boxes * (uint32_t)(sa.box * D));
+          __syncwarp();
+          if (go_mine) {
+            const int key = (jb + j) * BLK + 16 * grp;
+            sm100::tma_load_4d(sm + (v ? S::SV : S::SK) + h * S::SLOT + (grp & 3) * 16 * D, v ? &tv : &tk, full, 0,
+                               sa.t_shift >= 0 ? key & (a.c.T - 1) : key % a.c.T, w.head, id0);
+          }
+          ++staged;
+        }
+        id0 = id1;
+        id1 = id2;
+        sc0 = sc1;
+      }
+      // every copy has landed before the block's shared memory goes: the last use of each slot
+      if (lane == 0)
+        for (int q = 0; q < 4; ++q) {
+          const int uses = (staged + 3 - q) / 4;
+          if (uses > 0) sm100::mbar_wait_unwind(q >= 2 ? &sv_full[q & 1] : &sk_full[q & 1], (uint32_t)((uses - 1) & 1));
+        }
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------- MMA issuer ----
+      constexpr uint32_t idesc_qk = sm100::instr_desc(0, false, false, BLK, BLK);
+      constexpr uint32_t idesc_pv = sm100::instr_desc(0, false, true, BLK, D);
+      bool ok = n > 0 && sm100::mbar_wait(q_full, 0, abort_flag, a.err);
+      sm100::tc_fence_after();
+      const uint32_t d_hi = sm100::smem_desc_hi(1024);
+      uint32_t q_lo[kTiles], k_lo[2], v_lo[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        q_lo[i] = sm100::smem_desc_lo(sm100::smem_u32(sm + S::Q + i * S::TILE), 16);
+        k_lo[i] = sm100::smem_desc_lo(sm100::smem_u32(sm + S::K + i * S::TILE), 16);
+        v_lo[i] = sm100::smem_desc_lo(sm100::smem_u32(sm + S::V + i * S::TILE), S::SUB);
+      }
+      // S_t(j) = Q_t K_j^T; K_j's first user waits for it, its last one releases it.
+      auto issue_s = [&](int t, int j) -> bool {
+        const int st = j & 1;
+        if (t == 0 || j >= n_t[0]) {
+          if (!sm100::mbar_wait(&k_full[st], (uint32_t)((j >> 1) & 1), abort_flag, a.err)) return false;
+          sm100::tc_fence_after();
+        }
+        if (lane == 0) {
+          const uint32_t a0 = q_lo[t], b0 = k_lo[st], d = tmem + kSCol + 128u * t;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * S::SUB + (kk & 3) * 32) >> 4;
+            if (kk == 0) sm100::mma_f16_lohi<false>(d, a0 + off, d_hi, b0 + off, d_hi, idesc_qk);
+            else sm100::mma_f16_lohi<true>(d, a0 + off, d_hi, b0 + off, d_hi, idesc_qk);
+          }
+          sm100::mma_commit(&s_full[t]);
+          if (t == 1 || j >= n_t[1]) sm100::mma_commit(&k_empty[st]);
+        }
+        __syncwarp();
+        return true;
+      };
+      // O_t += P_t(j) V_j, likewise.
+      auto issue_pv = [&](int t, int j) -> bool {
+        const int st = j & 1;
+        if (!sm100::mbar_wait(&p_full[t], (uint32_t)(j & 1), abort_flag, a.err)) return false;
+        if ((t == 0 || j >= n_t[0]) &&
+            !sm100::mbar_wait(&v_full[st], (uint32_t)((j >> 1) & 1), abort_flag, a.err))
+          return false;
+        sm100::tc_fence_after();
+        if (lane == 0) {
+          const uint32_t b0 = v_lo[st], p = tmem + kSCol + 128u * t, d = tmem + kOCol + 128u * t;
+#pragma unroll
+          for (int kk = 0; kk < BLK / 16; ++kk) {
+            const uint32_t off = (kk * 16 * 128) >> 4;
+            if (kk == 0 && j == 0) sm100::mma_f16_ts_lohi<false>(d, p + kk * 8, b0 + off, d_hi, idesc_pv);
+            else sm100::mma_f16_ts_lohi<true>(d, p + kk * 8, b0 + off, d_hi, idesc_pv);
+          }
+          sm100::mma_commit(&pv_done[t]);
+          if (t == 1 || j >= n_t[1]) sm100::mma_commit(&v_empty[st]);
+        }
+        __syncwarp();
+        return true;
+      };
+      if (ok && n_t[0] > 0) ok = issue_s(0, 0);
+      if (ok && n_t[1] > 0) ok = issue_s(1, 0);
+      for (int j = 0; ok && j < n; ++j) {
+        if (j < n_t[0]) {
+          ok = issue_pv(0, j);
+          if (ok && j + 1 < n_t[0]) ok = issue_s(0, j + 1);
+        }
+        if (ok && j < n_t[1]) {
+          ok = issue_pv(1, j);
+          if (ok && j + 1 < n_t[1]) ok = issue_s(1, j + 1);
+        }
+      }
+      if (lane == 0) {
+        sm100::mma_commit(done_bar);
+        sm100::mbar_wait_unwind(done_bar, 0);
+      }
+      __syncwarp();
+    }
+  } else if (warp < kSoftBase) {
+    // ----------------------------------------------------------------- widening ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
+    const int cw = warp - kConvBase, row = row_of<D>(lane >> 2), v = lane & 3;
+    constexpr int HALVES = D / 64;              // 4 vectors of 16 codes each
+    constexpr int STEPS = kHalf / 8 * HALVES / 4;  // steps of 8 keys x 4 vectors for each of 4 warps and half block
+    // One half block (64 keys) of K or V from a staging slot into the fp16 tile.
+    auto widen_half = [&](const uint8_t* slot, uint8_t* tile, const Info* I, bool is_v, int h, int key0) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const int step = cw * STEPS + s;
+        const int hv = step % HALVES, k8 = step / HALVES;  // half of the channels, group of 8 keys in the half block
+        const int kk = 8 * k8 + row;                       // key in the half block
+        uint32_t off;                                      // staged: TMA's swizzle
+        if constexpr (D == 128) off = kk * 128 + (((4 * hv + v) ^ (kk & 7)) << 4);
+        else off = kk * 64 + ((v ^ ((kk >> 1) & 3)) << 4);
+        const int g = 4 * h + (k8 >> 1);
+        uint4 c = make_uint4(0, 0, 0, 0);
+        const bool there = !((I->holes >> g) & 1) && key0 + kk < k_end;
+        if (there) c = *reinterpret_cast<const uint4*>(slot + off);
+        uint32_t r[8];
+        const uint32_t cw4[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) widen4<CODE>(cw4[i], r[2 * i], r[2 * i + 1]);
+        const float f = is_v ? I->vr[g] : I->kr[g];  // the same for the whole warp
+        if (f != 1.f) {
+          const __half2 f2 = __float2half2_rn(there ? f : 0.f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) r[i] = mul2(r[i], f2);
+        }
+        uint8_t* dst = tile + hv * S::SUB + (64 * h + kk) * 128;
+        *reinterpret_cast<uint4*>(dst + (((2 * v) ^ (kk & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+        *reinterpret_cast<uint4*>(dst + (((2 * v + 1) ^ (kk & 7)) << 4)) = make_uint4(r[4], r[5], r[6], r[7]);
+      }
+    };
+    bool ok = true;
+    for (int j = 0; ok && j < n; ++j) {
+      const int st = j & 1;
+      const Info* I = &info[j % kInfo];
+      for (int q = 0; ok && q < 4; ++q) {
+        const bool is_v = q >= 2;
+        const int h = q & 1;
+        if (h == 0)
+          ok = sm100::mbar_wait(is_v ? &v_empty[st] : &k_empty[st], (uint32_t)(((j >> 1) & 1) ^ 1), abort_flag, a.err);
+        if (q == 0 && ok) ok = sm100::mbar_wait(&info_full[j % kInfo], (uint32_t)((j / kInfo) & 1), abort_flag, a.err);
+        if (ok) ok = sm100::mbar_wait(is_v ? &sv_full[h] : &sk_full[h], (uint32_t)(j & 1), abort_flag, a.err);
+        if (!ok) break;
+        widen_half(sm + (is_v ? S::SV : S::SK) + h * S::SLOT, sm + (is_v ? S::V : S::K) + st * S::TILE, I, is_v, h,
+                   (jb + j) * BLK + 64 * h);
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(is_v ? &sv_empty[h] : &sk_empty[h]);
+        if (h == 1) {
+          fence_async_smem();
+          sm100::mbar_arrive(is_v ? &v_full[st] : &k_full[st]);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    const int t = (warp - kSoftBase) >> 2;
+    const int wq = warp & 3;                          // TMEM lane quarter
+    const int rt = t * BLK + wq * 32 + lane;          // row in the block's pair of tiles
+    const int r = r0 + rt;
+    const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
+    const uint32_t s_tmem = tmem + kSCol + 128u * t + lane_addr;
+    const uint32_t o_tmem = tmem + kOCol + 128u * t + lane_addr;
+    // this row's query, scaled, into its swizzled tile row
+    float rowsc;
+    {
+      const T* qp = reinterpret_cast<const T*>(a.q);
+      if (r < a.rows)
+        qp += (int64_t)w.b * a.q_b + (int64_t)(w.head * a.group + r % a.group) * a.q_h + (int64_t)(r / a.group) * a.q_s;
+      uint32_t x[D / 2];  // pairs as loaded
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        uint4 y = make_uint4(0, 0, 0, 0);
+        if (r < a.rows) {
+          if (sa.q_vec) {
+            y = *reinterpret_cast<const uint4*>(qp + 8 * i);
+          } else {
+            ew::Vec<T, 8> e;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e.v[k] = qp[8 * i + k];
+            y = *reinterpret_cast<const uint4*>(&e);
+          }
+        }
+        x[4 * i] = y.x; x[4 * i + 1] = y.y; x[4 * i + 2] = y.z; x[4 * i + 3] = y.w;
+      }
+      auto lo_hi = [](uint32_t u) -> float2 {
+        const ew::Vec<T, 2> e = *reinterpret_cast<const ew::Vec<T, 2>*>(&u);
+        return make_float2(cvt<float>(e.v[0]), cvt<float>(e.v[1]));
+      };
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) {
+        const float2 f = lo_hi(x[i]);
+        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
+      const int be = (int)(__float_as_uint(amax) >> 23);
+      const int e = be == 255 ? 0 : min(max(141 - be, -110), 110);  // amax * 2^e in [2^14, 2^15)
+      const float up = a.scale < 0.f ? -pow2(e) : pow2(e);          // scores' factor stays positive
+      rowsc = fabsf(a.scale) * kLog2eF * pow2(-e);
+      uint8_t* q = sm + S::Q + t * S::TILE + (wq * 32 + lane) * 128;
+      const int sw = lane & 7;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        uint32_t y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = lo_hi(x[4 * i + k]);
+          y[k] = pack_f16(f.x * up, f.y * up);
+        }
+        *reinterpret_cast<uint4*>(q + (i >> 3) * S::SUB + (((i & 7) ^ sw) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+      }
+      fence_async_smem();
+      sm100::mbar_arrive(q_full);
+    }
+    const int mine = n_t[t];
+    const int kmax = r < a.rows ? last_key(a, len, start, r / a.group) : -1;
+    float m_used = -INFINITY, l = 0.f, vref = 1.f;
+    bool ok = true;
+    for (int j = 0; j < mine; ++j) {
+      const int k0 = (jb + j) * BLK;
+      if (!sm100::mbar_wait(&info_full[j % kInfo], (uint32_t)((j / kInfo) & 1), abort_flag, a.err)) { ok = false; break; }
+      const Info* I = &info[j % kInfo];
+      // positive even for a zero scale (or one that underflows): masked scores are -inf, and -inf * 0
+      // would be NaN
+      float sc = rowsc * I->kref;
+      if (sc < 1.17549435e-38f) sc = 1.17549435e-38f;
+      const float vfac = I->vfac;
+      const uint32_t holes = I->holes;
+      vref = I->vref;
+      if (!sm100::mbar_wait(&s_full[t], (uint32_t)(j & 1), abort_flag, a.err)) { ok = false; break; }
+      sm100::tc_fence_after();
+      uint32_t sr[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sm100::tmem_ld_32x32b_x32(s_tmem + c * 32, sr[c]);
+      sm100::tmem_ld_wait();
+      if (k0 + BLK - 1 > kmax || holes != 0) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (k0 + c * 32 + i > kmax || ((holes >> (2 * c + (i >> 4))) & 1)) sr[c][i] = __float_as_uint(-INFINITY);
+      }
+      // row max: eight independent chains of three-input maxima
+      float mx8[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t* v = &sr[k >> 1][(k & 1) * 16];
+        float m = max3f(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
+#pragma unroll
+        for (int i = 3; i + 1 < 16; i += 2) m = max3f(m, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        mx8[k] = fmaxf(m, __uint_as_float(v[15]));
+      }
+      const float mx = max3f(max3f(mx8[0], mx8[1], mx8[2]), max3f(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
+      const float m_blk = mx * sc;
+      const bool grow = m_blk > m_used + kRescaleThreshold;
+      const float m_prev = m_used;
+      if (grow) m_used = m_blk;
+      const float m_ref = m_used == -INFINITY ? 0.f : m_used;
+      const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(-m_ref, -m_ref);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), sc2, nm2);
+          x.x = sm100::ex2_approx(x.x);
+          x.y = sm100::ex2_approx(x.y);
+          sr[c][2 * i] = __float_as_uint(x.x);
+          sr[c][2 * i + 1] = __float_as_uint(x.y);
+          pk[i] = pack_f16(x.x, x.y);
+        }
+        sm100::tmem_st_32x32b_x16(s_tmem + c * 16, pk);
+      }
+      float alpha = 1.f;
+      if (__any_sync(0xffffffffu, (grow || vfac != 1.f) && j > 0)) {
+        alpha = grow ? exp2f(m_prev - m_blk) : 1.f;
+        // PV_t(j-1) (and, by commit order, every earlier PV of this tile) must be complete.
+        if (!sm100::mbar_wait(&pv_done[t], (uint32_t)((j - 1) & 1), abort_flag, a.err)) { ok = false; break; }
+        sm100::tc_fence_after();
+        const float f = alpha * vfac;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t x[32];
+          sm100::tmem_ld_32x32b_x32(o_tmem + c * 32, x);
+          sm100::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+          sm100::tmem_st_32x32b_x32(o_tmem + c * 32, x);
+        }
+      }
+      sm100::tmem_st_wait();
+      sm100::tc_fence_before();
+      sm100::mbar_arrive(&p_full[t]);
+      float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          sum[i & 3] =
+              __fadd2_rn(sum[i & 3], make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])));
+      const float2 s2 = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+      l = l * alpha + (s2.x + s2.y);
+    }
+    if (ok && mine > 0) ok = sm100::mbar_wait(&pv_done[t], (uint32_t)((mine - 1) & 1), abort_flag, a.err);
+    sm100::tc_fence_after();
+    if (ok) {
+      const bool whole = sa.splits == 1;
+      const float f = !whole ? vref : l == 0.f ? 0.f : vref / l;
+      const bool none = l == 0.f;  // nothing seen (NaN is not 0)
+      float* part = nullptr;
+      T* op = nullptr;
+      if (r < a.rows) {
+        if (whole) {
+          op = reinterpret_cast<T*>(a.o) + (int64_t)w.b * a.o_b +
+               (int64_t)(w.head * a.group + r % a.group) * a.o_h + (int64_t)(r / a.group) * a.o_s;
+        } else {
+          part = a.part + (int64_t)blockIdx.x * slot_floats(kTiles * BLK, D);
+          part[(int64_t)kTiles * BLK * D + 2 * rt] = m_used;
+          part[(int64_t)kTiles * BLK * D + 2 * rt + 1] = l;
+          part += (int64_t)rt * D;
+        }
+      }
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t x[32];
+        if (mine > 0) {  // the same for the whole warp
+          sm100::tmem_ld_32x32b_x32(o_tmem + c * 32, x);
+          sm100::tmem_ld_wait();
+        }
+        if (mine == 0 || none) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = 0u;
+        }
+        if (op != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            ew::Vec<T, 8> y;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y.v[e] = cvt<T>(__uint_as_float(x[i + e]) * f);
+            if (sa.o_vec) {
+              *reinterpret_cast<ew::Vec<T, 8>*>(op + c * 32 + i) = y;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) op[c * 32 + i + e] = y.v[e];
+            }
+          }
+        } else if (part != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(part + c * 32 + i) =
+                make_float4(__uint_as_float(x[i]) * f, __uint_as_float(x[i + 1]) * f, __uint_as_float(x[i + 2]) * f,
+                            __uint_as_float(x[i + 3]) * f);
+        }
+      }
+    }
+  }
+
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the splits of every row, one warp a row, as combine_kernel does.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv_split_combine(AttnArgs a, int splits) {
+  constexpr int E = D / 32;  // channels of a lane
+  using V = ew::Vec<float, E>;
+  const int lane = threadIdx.x & 31;
+  const int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);  // (segment, row), segments as where_is orders them
+  const int rows = kTiles * BLK;
+  const int64_t seg = job / rows;
+  const int rt = (int)(job % rows);
+  if (seg >= (int64_t)a.nb * a.tiles * a.c.H) return;
+  const Where w = where_is(a, 1, seg);
+  const int r = w.tile * rows + rt;
+  if (r >= a.rows) return;
+  grid_dependency_wait();
+  const int64_t slot = slot_floats(rows, D);
+  const float* base = a.part + seg * splits * slot;
+  const int64_t stat = (int64_t)rows * D + 2 * rt;
+  float M = -INFINITY;
+  for (int c = lane; c < splits; c += 32) M = fmaxf(M, base[c * slot + stat]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float ref = M == -INFINITY ? 0.f : M;
+  float L = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int cb = 0; cb < splits; cb += 32) {
+    float f = 0.f;
+    if (cb + lane < splits) {
+      const float* s = base + (cb + lane) * slot + stat;
+      f = exp2f(s[0] - ref);
+      L = fmaf(s[1], f, L);
+    }
+    const int k_n = min(32, splits - cb);
+    for (int k0 = 0; k0 < k_n; k0 += 4) {
+      V v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k0 + k < k_n) v[k] = *reinterpret_cast<const V*>(base + (cb + k0 + k) * slot + (int64_t)rt * D + lane * E);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
+        if (k0 + k < k_n)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(v[k].v[e], fk, acc[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  T* o = reinterpret_cast<T*>(a.o) + (int64_t)w.b * a.o_b + (int64_t)(w.head * a.group + r % a.group) * a.o_h +
+         (int64_t)(r / a.group) * a.o_s + lane * E;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = cvt<T>(L == 0.f ? 0.f : acc[e] * inv);
+}
+
+template <typename T, int CODE, int D>
+int go(const AttnArgs& a, int splits, cudaStream_t st) {
+  auto k = prompt_kernel<T, CODE, D>;
+  static std::atomic<int> regs_ok{0};
+  if (regs_ok.load() == 0) {
+    cudaFuncAttributes fa;
+    NTB_CUDA(cudaFuncGetAttributes(&fa, k));
+    regs_ok.store(fa.numRegs >= kLaunchRegs ? 1 : -1);
+  }
+  NTB_UNSUP(regs_ok.load() == 1, "attention kernel built with fewer than %d registers per thread", kLaunchRegs);
+  NTB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL));
+  SplitArgs sa;
+  sa.splits = splits;
+  sa.box = 16;
+  while (sa.box < kHalf && a.c.T % (2 * sa.box) == 0) sa.box *= 2;
+  sa.t_shift = -1;
+  if ((a.c.T & (a.c.T - 1)) == 0)
+    for (sa.t_shift = 0; (1 << sa.t_shift) < a.c.T;) ++sa.t_shift;
+  sa.q_vec = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && (a.q_b % 8 == 0 || a.table.B == 1) &&
+             (a.q_h % 8 == 0 || a.Hq == 1) && (a.q_s % 8 == 0 || a.Sq == 1);
+  sa.o_vec = reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && (a.o_b % 8 == 0 || a.table.B == 1) &&
+             (a.o_h % 8 == 0 || a.Hq == 1) && (a.o_s % 8 == 0 || a.Sq == 1);
+  CUtensorMap tk, tv;
+  int rc;
+  if ((rc = code_map(&tk, a.c.key, a.c, a.c.k_t, a.c.k_h, a.c.k_p, sa.box)) != NTB_OK) return rc;
+  if ((rc = code_map(&tv, a.c.value, a.c, a.c.v_t, a.c.v_h, a.c.v_p, sa.box)) != NTB_OK) return rc;
+  const int64_t segs = (int64_t)a.nb * a.tiles * a.c.H, grid = segs * splits;
+  NTB_UNSUP(grid <= 0x7fffffffLL && segs * 64 <= 0x7fffffffLL, "kv_attention: too many query rows");
+  k<<<(unsigned)grid, kThreads, Smem<D>::TOTAL, st>>>(tk, tv, a, sa);
+  NTB_LAUNCH_CHECK();
+  if (splits > 1)
+    NTB_CUDA(launch_dependent(kv_split_combine<T, D>, dim3((unsigned)(segs * kTiles * BLK / 4)), dim3(128), 0, st, a,
+                              splits));
+  return NTB_OK;
+}
+
+// Blocks that share a segment's keys: as many as one wave of one block an SM holds, each with at
+// least four key blocks of a full table.
+int splits_of(const AttnArgs& a) {
+  const int64_t segs = (int64_t)std::min(a.table.B, kMaxBatch) * a.tiles * a.c.H;
+  const int64_t cap = ((int64_t)a.table.M * a.c.T + 4 * BLK - 1) / (4 * BLK);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / segs, cap));
+}
+
+}  // namespace
+
+void prompt_plan(AttnArgs* a) {
+  a->tile = kTiles * BLK;
+  a->tiles = (a->rows + a->tile - 1) / a->tile;
+  a->unit = BLK;
+  const int splits = splits_of(*a);
+  // combine_kernel is not used: G only sizes the workspace (two slots for each unit of G)
+  a->G = splits > 1 ? (int)(((int64_t)std::min(a->table.B, kMaxBatch) * a->tiles * a->c.H * splits + 1) / 2) : 0;
+}
+
+int prompt_launch(const AttnArgs& a, int dtype, cudaStream_t st) {
+  const int splits = splits_of(a);
+  auto by_d = [&](auto t, auto code) -> int {
+    using T = decltype(t);
+    constexpr int CODE = decltype(code)::value;
+    return a.c.D == 128 ? go<T, CODE, 128>(a, splits, st) : go<T, CODE, 64>(a, splits, st);
+  };
+  using E = std::integral_constant<int, NTB_F8E4M3>;
+  using I = std::integral_constant<int, NTB_I8>;
+  if (dtype == NTB_BF16)
+    return a.c.code == NTB_F8E4M3 ? by_d(__nv_bfloat16{}, E{}) : by_d(__nv_bfloat16{}, I{});
+  return a.c.code == NTB_F8E4M3 ? by_d(__half{}, E{}) : by_d(__half{}, I{});
+}
+
+}  // namespace kv
+}  // namespace ntb

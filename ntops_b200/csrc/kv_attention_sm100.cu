@@ -381,27 +381,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int cw = warp - kConvBase, row = row_of<D>(lane >> 2), v = lane & 3;
     constexpr int HALVES = D / 64;              // 4 vectors of 16 codes each
     constexpr int STEPS = kHalf / 8 * HALVES / 4;  // steps of 8 keys x 4 vectors for each of 4 warps and half block
-    // One half block (64 keys) of K or V from a staging slot into the fp16 tile.
+    // One half block (64 keys) of K or V from a staging slot into the fp16 tile: 16 keys, one
+    // group, a warp; the loads of all its vectors are in flight together.
     auto widen_half = [&](const uint8_t* slot, uint8_t* tile, const Info* I, bool is_v, int h, int key0) {
+      const int g = 4 * h + cw;
+      const float f = is_v ? I->vr[g] : I->kr[g];
+      const bool hole = (I->holes >> g) & 1;
+      uint4 c[STEPS];
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        const int step = cw * STEPS + s;
-        const int hv = step % HALVES, k8 = step / HALVES;  // half of the channels, group of 8 keys in the half block
-        const int kk = 8 * k8 + row;                       // key in the half block
-        uint32_t off;                                      // staged: TMA's swizzle
+        const int kk = 16 * cw + 8 * (s / HALVES) + row, hv = s % HALVES;  // key in the half block, half of the channels
+        uint32_t off;                                                      // staged: TMA's swizzle
         if constexpr (D == 128) off = kk * 128 + (((4 * hv + v) ^ (kk & 7)) << 4);
         else off = kk * 64 + ((v ^ ((kk >> 1) & 3)) << 4);
-        const int g = 4 * h + (k8 >> 1);
-        uint4 c = make_uint4(0, 0, 0, 0);
-        const bool there = !((I->holes >> g) & 1) && key0 + kk < k_end;
-        if (there) c = *reinterpret_cast<const uint4*>(slot + off);
-        uint32_t r[8];
-        const uint32_t cw4[4] = {c.x, c.y, c.z, c.w};
+        c[s] = *reinterpret_cast<const uint4*>(slot + off);
+      }
+      if (hole || key0 + 16 * cw + 16 > k_end) {  // what is no key may be anything
 #pragma unroll
-        for (int i = 0; i < 4; ++i) widen4<CODE>(cw4[i], r[2 * i], r[2 * i + 1]);
-        const float f = is_v ? I->vr[g] : I->kr[g];  // the same for the whole warp
+        for (int s = 0; s < STEPS; ++s)
+          if (hole || key0 + 16 * cw + 8 * (s / HALVES) + row >= k_end) c[s] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const int kk = 16 * cw + 8 * (s / HALVES) + row, hv = s % HALVES;
+        uint32_t r[8];
+        widen4<CODE>(c[s].x, r[0], r[1]);
+        widen4<CODE>(c[s].y, r[2], r[3]);
+        widen4<CODE>(c[s].z, r[4], r[5]);
+        widen4<CODE>(c[s].w, r[6], r[7]);
         if (f != 1.f) {
-          const __half2 f2 = __float2half2_rn(there ? f : 0.f);
+          const __half2 f2 = __float2half2_rn(hole ? 0.f : f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) r[i] = mul2(r[i], f2);
         }

@@ -149,7 +149,7 @@ inline int code_map(CUtensorMap* map, uint8_t* base, const Layer& c, int64_t s_t
 // Whether the tensor-core kernels take these operands (16-bit queries, head_dim 64 or 128, pages of
 // whole 16-key groups, strides that TMA accepts).
 bool tensor_cores_take(const AttnArgs& a, int dtype);
-// Up to 16 packed rows (kv_attention_decode.cu): plan fills tile, tiles, unit and G.
+// Up to 32 packed rows (kv_attention_decode.cu): plan fills tile, tiles, unit and G.
 int decode_plan(AttnArgs* a, int dtype);
 int decode_launch(const AttnArgs& a, int dtype, cudaStream_t st);
 // More rows (kv_attention_sm100.cu); joins its own pieces.

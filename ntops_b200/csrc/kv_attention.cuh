@@ -86,6 +86,12 @@ __device__ __forceinline__ void prefix_units(const AttnArgs& a, int* pre) {
   __syncthreads();
 }
 
+// a / b for a >= 0, b > 0: in 32 bits where they suffice (a 64-bit division is some hundred
+// instructions, and the ones below stand before a block's first load).
+__device__ __forceinline__ int64_t quotient(int64_t a, int b) {
+  return (uint64_t)a <= 0xFFFFFFFFull ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // The line of units and its division among the blocks.
 struct Line {
   int64_t total;
@@ -95,7 +101,7 @@ struct Line {
     total = (int64_t)pre[a.nb] * segs;
     blocks = (int)min((int64_t)a.G, total);
   }
-  __device__ __forceinline__ int64_t begin(int i) const { return total * i / blocks; }
+  __device__ __forceinline__ int64_t begin(int i) const { return quotient(total * i, blocks); }
   // the block whose share holds unit u
   __device__ __forceinline__ int owner(int64_t u) const { return (int)(((u + 1) * blocks - 1) / total); }
 };
@@ -118,7 +124,7 @@ __device__ __forceinline__ Piece piece_at(const AttnArgs& a, const Line& line, c
   }
   const int units = pre[x + 1] - pre[x];
   const int64_t rem = pos - (int64_t)pre[x] * line.segs;
-  const int seg = (int)(rem / units);
+  const int seg = (int)quotient(rem, units);
   Piece p;
   p.b = a.b0 + x;
   p.tile = seg / a.c.H;

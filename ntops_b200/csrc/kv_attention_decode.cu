@@ -100,7 +100,7 @@ struct Cfg {
   static constexpr int REC = STAGES * STAGE;         // {ks, vs, page id} of a stage's 8 groups of 16 keys
   static constexpr int BUF = REC + STAGES * 128;     // float [8 RT][OS], then max, sum [8 RT]
   static constexpr int BAR = BUF + 8 * RT * (OS + 2) * 4;
-  static constexpr int PRE = BAR + 16 * STAGES + 16;
+  static constexpr int PRE = BAR + 32 * STAGES + 16;
   static constexpr int SLACK = 1024;                 // to align the dynamic shared memory
   static_assert(STAGE % 1024 == 0 && BAR % 16 == 0, "alignment");
 };
@@ -145,15 +145,19 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
   float* buf = reinterpret_cast<float*>(dyn + C::BUF);
   float* buf_m = buf + ROWS * C::OS;
   float* buf_l = buf_m + ROWS;
-  uint64_t* full = reinterpret_cast<uint64_t*>(dyn + C::BAR);
-  uint64_t* empty = full + C::STAGES;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + C::STAGES);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(dyn + C::BAR);
+  uint64_t* k_empty = k_full + C::STAGES;
+  uint64_t* v_full = k_empty + C::STAGES;
+  uint64_t* v_empty = v_full + C::STAGES;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(v_empty + C::STAGES);
   int* pre = reinterpret_cast<int*>(dyn + C::PRE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      sm100::mbar_init(&full[s], 1);
-      sm100::mbar_init(&empty[s], kConsumers);
+      sm100::mbar_init(&k_full[s], 1);
+      sm100::mbar_init(&k_empty[s], kConsumers);
+      sm100::mbar_init(&v_full[s], 1);
+      sm100::mbar_init(&v_empty[s], kConsumers);
     }
     *abort_flag = 0;
     sm100::fence_mbar_init();
@@ -204,36 +208,37 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
     Unit w1 = advance();
     int id1 = page_id(w1);
     float sc0 = page_scale(w0, id0);
-    int issued = 0;
+    int issued = 0, armed = 0;  // units; slots of K and V, in turn
     for (; w0.b >= 0; ++issued) {
       const int st = issued % C::STAGES;
+      const uint32_t phase = (uint32_t)((issued / C::STAGES - 1) & 1);
+      const int key = w0.key0 + 16 * grp;
+      const int in_page = t_shift >= 0 ? key & (a.c.T - 1) : key % a.c.T;
       int ok = 1;
-      if (lane == 0 && issued >= C::STAGES)
-        ok = sm100::mbar_wait(&empty[st], (uint32_t)((issued / C::STAGES - 1) & 1), abort_flag, a.err);
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-      const bool mine = first && id0 >= 0;
-      const unsigned boxes = __ballot_sync(0xffffffffu, mine);
-      // The stage's one arrival comes after the scales are written; the copies' bytes are
-      // announced before the first can land.
-      if (lane == 0)
-        asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(sm100::smem_u32(&full[st])),
-                     "r"((uint32_t)__popc(boxes) * (uint32_t)(box * D))
-                     : "memory");
-      __syncwarp();
-      if (mine) {
-        const int key = w0.key0 + 16 * grp;
-        const int in_page = t_shift >= 0 ? key & (a.c.T - 1) : key % a.c.T;
-        sm100::tma_load_4d(dyn + st * C::STAGE + (is_v ? C::K_BYTES : 0) + 16 * grp * D, is_v ? &tv : &tk, &full[st], 0,
-                           in_page, w0.head, id0);
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {  // K, then V: their slots are free at different times
+        uint64_t* full = v ? &v_full[st] : &k_full[st];
+        if (lane == 0 && issued >= C::STAGES)
+          ok = sm100::mbar_wait(v ? &v_empty[st] : &k_empty[st], phase, abort_flag, a.err);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        if (v == 0 && lane < 16) {  // 16-byte records {ks, vs, id, -}, read with K
+          float* rec = reinterpret_cast<float*>(dyn + C::REC + st * 128) + grp * 4;
+          rec[is_v ? 1 : 0] = sc0;
+          if (!is_v) reinterpret_cast<int*>(rec)[2] = id0;
+        }
+        const bool mine = first && is_v == (v == 1) && id0 >= 0;
+        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive_expect_tx(full, boxes * (uint32_t)(box * D));
+        __syncwarp();
+        if (mine)
+          sm100::tma_load_4d(dyn + st * C::STAGE + (v ? C::K_BYTES : 0) + 16 * grp * D, v ? &tv : &tk, full, 0, in_page,
+                             w0.head, id0);
+        ++armed;
       }
+      if (!ok) break;
       id1 = checked(id1);
-      if (lane < 16) {  // 16-byte records {ks, vs, id, -}
-        float* rec = reinterpret_cast<float*>(dyn + C::REC + st * 128) + grp * 4;
-        rec[is_v ? 1 : 0] = sc0;
-        if (!is_v) reinterpret_cast<int*>(rec)[2] = id0;
-      }
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&full[st]);
       const Unit w2 = advance();
       sc0 = page_scale(w1, id1);
       w0 = w1;
@@ -241,10 +246,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
       w1 = w2;
       id1 = page_id(w2);
     }
-    // every copy has landed before the block's shared memory goes
+    // every copy has landed before the block's shared memory goes: the last uses of each slot
     if (lane == 0)
-      for (int i = max(issued - C::STAGES, 0); i < issued; ++i)
-        sm100::mbar_wait_unwind(&full[i % C::STAGES], (uint32_t)((i / C::STAGES) & 1));
+      for (int i = max(armed - 2 * C::STAGES, 0); i < armed; ++i)
+        sm100::mbar_wait_unwind(i & 1 ? &v_full[(i / 2) % C::STAGES] : &k_full[(i / 2) % C::STAGES],
+                                (uint32_t)((i / 2 / C::STAGES) & 1));
     return;
   }
 
@@ -333,138 +339,152 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
     }
     for (int u = pc.u0; u < pc.u1; ++u, ++it) {
       const int st = it % C::STAGES;
-      if (ok) ok = sm100::mbar_wait(&full[st], (uint32_t)((it / C::STAGES) & 1), abort_flag, a.err);
+      const uint32_t phase = (uint32_t)((it / C::STAGES) & 1);
+      if (ok) ok = sm100::mbar_wait(&k_full[st], phase, abort_flag, a.err);
       if (!ok) break;
       const int kw = u * kUnit + 32 * warp;  // column c of tile n is key kw + 8n + row_of(c)
-      if (kw < k_end) {
-        const uint4 rec0 = lds16(rec_off + st * 128), rec1 = lds16(rec_off + st * 128 + 16);
-        const float ks[2] = {__uint_as_float(rec0.x), __uint_as_float(rec1.x)};
-        const float vs[2] = {__uint_as_float(rec0.y), __uint_as_float(rec1.y)};
-        const bool hole[2] = {(int)rec0.z < 0, (int)rec1.z < 0};  // or a group past the last key
-        // ----------------------------------------------------------- S = Q K^T ----
-        float s[4][4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-        // keys innermost: four independent accumulators in turn
-#pragma unroll
-        for (int h = 0; h < H64; ++h) {
-          uint4 kr[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) kr[n] = lds16(k_off[h] + st * C::STAGE + 8 * n * D);
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const uint32_t c = w == 0 ? kr[n].x : w == 1 ? kr[n].y : w == 2 ? kr[n].z : kr[n].w;
-              uint32_t b0, b1;
-              widen4<CODE>(bias<CODE>(c), b0, b1);
-              mma_f16(s[n], qa[0][h * 4 + w][0], RT == 2 ? qa[RT - 1][h * 4 + w][0] : 0u, qa[0][h * 4 + w][1],
-                      RT == 2 ? qa[RT - 1][h * 4 + w][1] : 0u, b0, b1);
-            }
+      if (kw >= k_end) {  // nothing for this warp: it only hands the stage on
+        __syncwarp();
+        if (lane == 0) {
+          sm100::mbar_arrive(&k_empty[st]);
+          sm100::mbar_arrive(&v_empty[st]);
         }
-        // ------------------------------------------------------------- softmax ----
-        const bool edge = kw + 31 > k_low || hole[0] || hole[1];  // the same for every lane
-        float alpha[RT];
-        bool grown = false;
+        continue;
+      }
+      const uint4 rec0 = lds16(rec_off + st * 128), rec1 = lds16(rec_off + st * 128 + 16);
+      const float ks[2] = {__uint_as_float(rec0.x), __uint_as_float(rec1.x)};
+      const float vs[2] = {__uint_as_float(rec0.y), __uint_as_float(rec1.y)};
+      const bool hole[2] = {(int)rec0.z < 0, (int)rec1.z < 0};  // or a group past the last key
+      // ----------------------------------------------------------- S = Q K^T ----
+      float s[4][4];
 #pragma unroll
-        for (int x = 0; x < RT; ++x) {
-          float mb = -INFINITY;
-          const float sc[2] = {rowsc[x] * ks[0], rowsc[x] * ks[1]};
+      for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      // keys innermost: four independent accumulators in turn
+#pragma unroll
+      for (int h = 0; h < H64; ++h) {
+        uint4 kr[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) kr[n] = lds16(k_off[h] + st * C::STAGE + 8 * n * D);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint32_t c = w == 0 ? kr[n].x : w == 1 ? kr[n].y : w == 2 ? kr[n].z : kr[n].w;
+            uint32_t b0, b1;
+            widen4<CODE>(bias<CODE>(c), b0, b1);
+            mma_f16(s[n], qa[0][h * 4 + w][0], RT == 2 ? qa[RT - 1][h * 4 + w][0] : 0u, qa[0][h * 4 + w][1],
+                    RT == 2 ? qa[RT - 1][h * 4 + w][1] : 0u, b0, b1);
+          }
+      }
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&k_empty[st]);  // K's next unit may come while this one goes on
+      // ------------------------------------------------------------- softmax ----
+      const bool edge = kw + 31 > k_low || hole[0] || hole[1];  // the same for every lane
+      float mb[RT];
+      bool grow = false;
+#pragma unroll
+      for (int x = 0; x < RT; ++x) {
+        const float sc[2] = {rowsc[x] * ks[0], rowsc[x] * ks[1]};
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) s[n][2 * x + e] *= sc[n >> 1];
+        if (__builtin_expect(edge, 0)) {
 #pragma unroll
           for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float v = s[n][2 * x + e] * sc[n >> 1];
-              if (edge && (hole[n >> 1] || kw + 8 * n + kc[e] > kmax[x])) v = -INFINITY;
-              s[n][2 * x + e] = v;
-              mb = fmaxf(mb, v);
-            }
-          mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
-          mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
-          alpha[x] = 1.f;
-          if (mb > m[x] + kGrow) {
-            alpha[x] = exp2f(m[x] - mb);  // 0 at the first block that the row sees
-            m[x] = mb;
-            grown = true;
-          }
+            for (int e = 0; e < 2; ++e)
+              if (hole[n >> 1] || kw + 8 * n + kc[e] > kmax[x]) s[n][2 * x + e] = -INFINITY;
         }
-        const float vtop = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
+        mb[x] = fmaxf(fmaxf(fmaxf(s[0][2 * x], s[0][2 * x + 1]), fmaxf(s[1][2 * x], s[1][2 * x + 1])),
+                      fmaxf(fmaxf(s[2][2 * x], s[2][2 * x + 1]), fmaxf(s[3][2 * x], s[3][2 * x + 1])));
+        mb[x] = fmaxf(mb[x], __shfl_xor_sync(0xffffffffu, mb[x], 1));
+        mb[x] = fmaxf(mb[x], __shfl_xor_sync(0xffffffffu, mb[x], 2));
+        grow |= mb[x] > m[x] + kGrow;
+      }
+      const float vtop = fmaxf(fabsf(vs[0]), fabsf(vs[1]));  // the same for every lane
+      if (__builtin_expect(__any_sync(0xffffffffu, grow) || vtop > vref, 0)) {
         float vmul = 1.f;
-        if (vtop > vref) {  // the same for every lane
+        if (vtop > vref) {
           vmul = vref / vtop;
           vref = vtop;
           inv_vref = 1.f / vtop;
         }
-        if (__any_sync(0xffffffffu, grown) || vmul != 1.f) {
-#pragma unroll
-          for (int x = 0; x < RT; ++x) {
-            l[x] *= alpha[x];
-            // O^T's columns are rows 2t and 2t + 1, whose statistics lanes 8t and 8t + 4 hold
-            const float a0 = __shfl_sync(0xffffffffu, alpha[x], 8 * t) * vmul;
-            const float a1 = __shfl_sync(0xffffffffu, alpha[x], 8 * t + 4) * vmul;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              o[x][i][0] *= a0;
-              o[x][i][1] *= a1;
-              o[x][i][2] *= a0;
-              o[x][i][3] *= a1;
-            }
-          }
-        }
-        uint32_t pb[RT][2][2];
-        const float f[2] = {vs[0] * inv_vref, vs[1] * inv_vref};
 #pragma unroll
         for (int x = 0; x < RT; ++x) {
-          const float ref = m[x] == -INFINITY ? 0.f : m[x];
+          float alpha = 1.f;
+          if (mb[x] > m[x] + kGrow) {
+            alpha = exp2f(m[x] - mb[x]);  // 0 at the first block that the row sees
+            m[x] = mb[x];
+          }
+          l[x] *= alpha;
+          // O^T's columns are rows 2t and 2t + 1, whose statistics lanes 8t and 8t + 4 hold
+          const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t) * vmul;
+          const float a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4) * vmul;
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const float p0 = sm100::ex2_approx(s[n][2 * x] - ref), p1 = sm100::ex2_approx(s[n][2 * x + 1] - ref);
-            l[x] += p0 + p1;
-            pb[x][n >> 1][n & 1] = pack_f16(p0 * f[n >> 1], p1 * f[n >> 1]);
+          for (int i = 0; i < MT; ++i) {
+            o[x][i][0] *= a0;
+            o[x][i][1] *= a1;
+            o[x][i][2] *= a0;
+            o[x][i][3] *= a1;
           }
         }
-        // ------------------------------------------------------- O^T += V^T P^T ----
+      }
+      uint32_t pb[RT][2][2];
+      const float f[2] = {vs[0] * inv_vref, vs[1] * inv_vref};
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t vr[4][VW];  // keys (column 2t, tile 2j), (2t + 1, 2j), (2t, 2j + 1), (2t + 1, 2j + 1)
+      for (int x = 0; x < RT; ++x) {
+        const float ref = m[x] == -INFINITY ? 0.f : m[x];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t at = v_off[k & 1] + st * C::STAGE + 8 * (2 * j + (k >> 1)) * D;
-            if constexpr (VW == 4) {
-              const uint4 x = lds16(at);
-              vr[k][0] = x.x; vr[k][1] = x.y; vr[k][VW - 2] = x.z; vr[k][VW - 1] = x.w;
-            } else {
-              const uint2 x = lds8(at);
-              vr[k][0] = x.x; vr[k][1] = x.y;
-            }
+        for (int n = 0; n < 4; ++n) {
+          const float p0 = sm100::ex2_approx(s[n][2 * x] - ref), p1 = sm100::ex2_approx(s[n][2 * x + 1] - ref);
+          l[x] += p0 + p1;
+          pb[x][n >> 1][n & 1] = pack_f16(p0 * f[n >> 1], p1 * f[n >> 1]);
+        }
+      }
+      ok = sm100::mbar_wait(&v_full[st], phase, abort_flag, a.err);
+      if (!ok) break;
+      // ------------------------------------------------------- O^T += V^T P^T ----
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t vr[4][VW];  // keys (column 2t, tile 2j), (2t + 1, 2j), (2t, 2j + 1), (2t + 1, 2j + 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t at = v_off[k & 1] + st * C::STAGE + 8 * (2 * j + (k >> 1)) * D;
+          if constexpr (VW == 4) {
+            const uint4 x = lds16(at);
+            vr[k][0] = x.x; vr[k][1] = x.y; vr[k][VW - 2] = x.z; vr[k][VW - 1] = x.w;
+          } else {
+            const uint2 x = lds8(at);
+            vr[k][0] = x.x; vr[k][1] = x.y;
           }
-          // what lies past the last key or in a hole's place is anything: 0 * NaN would not be 0
-          if (edge) {
+        }
+        // what lies past the last key or in a hole's place is anything: 0 * NaN would not be 0
+        if (__builtin_expect(edge, 0)) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (hole[j] || kw + 8 * (2 * j + (k >> 1)) + kc[k & 1] >= k_end)
+          for (int k = 0; k < 4; ++k)
+            if (hole[j] || kw + 8 * (2 * j + (k >> 1)) + kc[k & 1] >= k_end)
 #pragma unroll
-                for (int w = 0; w < VW; ++w) vr[k][w] = 0u;
-          }
+              for (int w = 0; w < VW; ++w) vr[k][w] = 0u;
+        }
 #pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            const uint32_t v0 = bias<CODE>(vr[0][w]), v1 = bias<CODE>(vr[1][w]);
-            const uint32_t v2 = bias<CODE>(vr[2][w]), v3 = bias<CODE>(vr[3][w]);
+        for (int w = 0; w < VW; ++w) {
+          const uint32_t v0 = bias<CODE>(vr[0][w]), v1 = bias<CODE>(vr[1][w]);
+          const uint32_t v2 = bias<CODE>(vr[2][w]), v3 = bias<CODE>(vr[3][w]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t x01 = __byte_perm(v0, v1, i ? 0x7362 : 0x5140);
-              const uint32_t x23 = __byte_perm(v2, v3, i ? 0x7362 : 0x5140);
-              uint32_t a0, a1, a2, a3;
-              widen4<CODE>(x01, a0, a1);
-              widen4<CODE>(x23, a2, a3);
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x01 = __byte_perm(v0, v1, i ? 0x7362 : 0x5140);
+            const uint32_t x23 = __byte_perm(v2, v3, i ? 0x7362 : 0x5140);
+            uint32_t a0, a1, a2, a3;
+            widen4<CODE>(x01, a0, a1);
+            widen4<CODE>(x23, a2, a3);
 #pragma unroll
-              for (int x = 0; x < RT; ++x) mma_f16(o[x][2 * w + i], a0, a1, a2, a3, pb[x][j][0], pb[x][j][1]);
-            }
+            for (int x = 0; x < RT; ++x) mma_f16(o[x][2 * w + i], a0, a1, a2, a3, pb[x][j][0], pb[x][j][1]);
           }
         }
       }
       __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&empty[st]);  // this warp is done with the stage
+      if (lane == 0) sm100::mbar_arrive(&v_empty[st]);
     }
     // --------------------------------------------- join the warps' results, 3 -> 2 -> 1 -> 0 ----
 #pragma unroll

@@ -96,10 +96,10 @@ struct Cfg {
   // allow three blocks, else two of three.
   static constexpr int BLOCKS = D == 128 ? (RT == 1 ? 3 : 2) : (RT == 1 ? 4 : 3);
   static constexpr int STAGES = D == 128 ? (RT == 1 ? 2 : 3) : 3;
-  static constexpr int OS = D + 4;                   // padded row of the merge buffer (floats)
   static constexpr int REC = STAGES * STAGE;         // {ks, vs, page id} of a stage's 8 groups of 16 keys
-  static constexpr int BUF = REC + STAGES * 128;     // float [8 RT][OS], then max, sum [8 RT]
-  static constexpr int BAR = BUF + 8 * RT * (OS + 2) * 4;
+  static constexpr int STAT = REC + STAGES * 128;    // max and sum of the four warps' rows
+  static constexpr int BAR = STAT + 4 * 8 * RT * 8;
+  static_assert(V_BYTES == kConsumers * 8 * D * 4, "the warps' results of 8 rows fill a V slot");
   static constexpr int PRE = BAR + 32 * STAGES + 16;
   static constexpr int SLACK = 1024;                 // to align the dynamic shared memory
   static_assert(STAGE % 1024 == 0 && BAR % 16 == 0, "alignment");
@@ -142,9 +142,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
   constexpr int ROWS = 8 * RT;
   extern __shared__ __align__(128) uint8_t dyn_raw[];
   uint8_t* dyn = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_raw) + 1023) & ~uintptr_t(1023));
-  float* buf = reinterpret_cast<float*>(dyn + C::BUF);
-  float* buf_m = buf + ROWS * C::OS;
-  float* buf_l = buf_m + ROWS;
+  float2* stat = reinterpret_cast<float2*>(dyn + C::STAT);  // [warp][ROWS]
   uint64_t* k_full = reinterpret_cast<uint64_t*>(dyn + C::BAR);
   uint64_t* k_empty = k_full + C::STAGES;
   uint64_t* v_full = k_empty + C::STAGES;
@@ -271,45 +269,40 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
   for (int64_t pos = lo; pos < hi;) {
     const Piece pc = piece_at(a, line, pre, pos, lo, hi);
     pos = pc.next;
-    const int len = row_length(a, pc.b), start = row_start(a, pc.b, len);
     const int r0 = pc.tile * ROWS;
     // ------------------------------------------------------------------- queries ----
     uint32_t qa[RT][H64 * 4][2];
     float rowsc[RT];  // scores of this lane's row(s): accumulator -> base-2 logits, without ks
     int kmax[RT];
+    const int len = row_length(a, pc.b), start = row_start(a, pc.b, len);  // in flight with the queries
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
       const int r = r0 + g + 8 * x;
-      float v[H64][16];
-      kmax[x] = r < a.rows ? last_key(a, len, start, r / a.group) : -1;
+      ew::Vec<T, 8> w[H64][2];
+#pragma unroll
+      for (int h = 0; h < H64; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(&w[h][e]) = make_uint4(0, 0, 0, 0);
       if (r < a.rows) {
         const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)pc.b * a.q_b +
                       (int64_t)(pc.head * a.group + r % a.group) * a.q_h + (int64_t)(r / a.group) * a.q_s + 16 * t;
 #pragma unroll
-        for (int h = 0; h < H64; ++h) {
-          if (q_vec) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const ew::Vec<T, 8> w = *reinterpret_cast<const ew::Vec<T, 8>*>(qp + 64 * h + 8 * e);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[h][8 * e + i] = cvt<float>(w.v[i]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[h][i] = cvt<float>(qp[64 * h + i]);
-          }
-        }
-      } else {
-#pragma unroll
         for (int h = 0; h < H64; ++h)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[h][i] = 0.f;
+          for (int e = 0; e < 2; ++e) {
+            if (q_vec) {
+              w[h][e] = *reinterpret_cast<const ew::Vec<T, 8>*>(qp + 64 * h + 8 * e);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[h][e].v[i] = qp[64 * h + 8 * e + i];
+            }
+          }
       }
       float amax = 0.f;
 #pragma unroll
       for (int h = 0; h < H64; ++h)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(v[h][i]));
+        for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(cvt<float>(w[h][i >> 3].v[i & 7])));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const int be = (int)(__float_as_uint(amax) >> 23);
@@ -320,9 +313,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
       for (int h = 0; h < H64; ++h)
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          qa[x][h * 4 + s][0] = pack_f16(v[h][4 * s] * up, v[h][4 * s + 1] * up);
-          qa[x][h * 4 + s][1] = pack_f16(v[h][4 * s + 2] * up, v[h][4 * s + 3] * up);
+          const ew::Vec<T, 8>& y = w[h][s >> 1];
+          const int k = 4 * (s & 1);
+          qa[x][h * 4 + s][0] = pack_f16(cvt<float>(y.v[k]) * up, cvt<float>(y.v[k + 1]) * up);
+          qa[x][h * 4 + s][1] = pack_f16(cvt<float>(y.v[k + 2]) * up, cvt<float>(y.v[k + 3]) * up);
         }
+      kmax[x] = r < a.rows ? last_key(a, len, start, r / a.group) : -1;
     }
     // every row of the tile sees the keys up to k_low; none sees a key at or past k_end
     const int k_low = last_key(a, len, start, r0 / a.group);
@@ -347,8 +343,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
         __syncwarp();
         if (lane == 0) {
           sm100::mbar_arrive(&k_empty[st]);
-          sm100::mbar_arrive(&v_empty[st]);
+          if (u + 1 < pc.u1) sm100::mbar_arrive(&v_empty[st]);
         }
+        if (u + 1 == pc.u1) ok = sm100::mbar_wait(&v_full[st], phase, abort_flag, a.err);
         continue;
       }
       const uint4 rec0 = lds16(rec_off + st * 128), rec1 = lds16(rec_off + st * 128 + 16);
@@ -484,103 +481,79 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
         }
       }
       __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&v_empty[st]);
+      if (lane == 0 && u + 1 < pc.u1) sm100::mbar_arrive(&v_empty[st]);
     }
-    // --------------------------------------------- join the warps' results, 3 -> 2 -> 1 -> 0 ----
+    // --------------------------------------------------- join the warps' results ----
+    // They meet in the last unit's V slot, which is handed back only then: 8 rows of fp32 from
+    // each warp fill it.  Row r's 16-byte chunk c lies at c ^ r.
+    const int last = (it + C::STAGES - 1) % C::STAGES;
+    float* slot = reinterpret_cast<float*>(dyn + last * C::STAGE + C::K_BYTES);
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[x][i][e] *= vref;
+      if (t == 0) stat[warp * ROWS + 8 * x + g] = make_float2(m[x], l[x]);
     }
-#pragma unroll 1
-    for (int w = kConsumers - 1; w > 0; --w) {
-      if (warp == w) {
 #pragma unroll
-        for (int x = 0; x < RT; ++x) {
-          if (t == 0) {
-            buf_m[8 * x + g] = m[x];
-            buf_l[8 * x + g] = l[x];
-          }
-          // channels 4 VW g + 2i (elements 0, 1) and + 2i + 1 (2, 3) of rows 2t and 2t + 1
+    for (int x = 0; x < RT; ++x) {
+      consumer_sync();  // every warp is through with the slot (x = 0: with its values)
+      // channels 4 VW g + 2i (elements 0, 1) and + 2i + 1 (2, 3) of rows 2t and 2t + 1
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int i = 0; i < MT; i += 2)
-              *reinterpret_cast<float4*>(&buf[(8 * x + 2 * t + e) * C::OS + 4 * VW * g + 2 * i]) =
-                  make_float4(o[x][i][e], o[x][i][2 + e], o[x][i + 1][e], o[x][i + 1][2 + e]);
-        }
-      }
+        for (int i = 0; i < MT; i += 2)
+          *reinterpret_cast<float4*>(slot + (warp * 8 + 2 * t + e) * D + (((VW * g + i / 2) ^ (2 * t + e)) << 2)) =
+              make_float4(o[x][i][e] * vref, o[x][i][2 + e] * vref, o[x][i + 1][e] * vref, o[x][i + 1][2 + e] * vref);
       consumer_sync();
-      if (warp == w - 1) {
+      // 16 threads a row, E channels each
+      constexpr int E = D / 16;
+      const int rr = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * (E / 4), rt = 8 * x + rr, r = r0 + rt;
+      float2 ml[kConsumers];
 #pragma unroll
-        for (int x = 0; x < RT; ++x) {
-          const float mo = buf_m[8 * x + g], M = fmaxf(m[x], mo), ref = M == -INFINITY ? 0.f : M;
-          const float fa = exp2f(m[x] - ref), fb = exp2f(mo - ref);
-          l[x] = l[x] * fa + buf_l[8 * x + g] * fb;
-          m[x] = M;
+      for (int w = 0; w < kConsumers; ++w) ml[w] = stat[w * ROWS + rt];
+      const float M = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), ref = M == -INFINITY ? 0.f : M;
+      float L = 0.f, acc[E];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float a0 = __shfl_sync(0xffffffffu, fa, 8 * t + 4 * e), b0 = __shfl_sync(0xffffffffu, fb, 8 * t + 4 * e);
+      for (int i = 0; i < E; ++i) acc[i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < MT; i += 2) {
-              const float4 y = *reinterpret_cast<const float4*>(&buf[(8 * x + 2 * t + e) * C::OS + 4 * VW * g + 2 * i]);
-              o[x][i][e] = fmaf(o[x][i][e], a0, y.x * b0);
-              o[x][i][2 + e] = fmaf(o[x][i][2 + e], a0, y.y * b0);
-              o[x][i + 1][e] = fmaf(o[x][i + 1][e], a0, y.z * b0);
-              o[x][i + 1][2 + e] = fmaf(o[x][i + 1][2 + e], a0, y.w * b0);
-            }
-          }
-        }
-        __syncwarp();  // it may write the buffer next
-      }
-    }
-    consumer_sync();  // warp 0 has read the buffer before the next piece writes it
-    if (warp == 0 && ok) {
+      for (int w = 0; w < kConsumers; ++w) {
+        const float f = exp2f(ml[w].x - ref);
+        L = fmaf(ml[w].y, f, L);
 #pragma unroll
-      for (int x = 0; x < RT; ++x) {
-        const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int rt = 8 * x + 2 * t + e, r = r0 + rt;
-          const float iv = __shfl_sync(0xffffffffu, inv, 8 * t + 4 * e);
-          const float L = __shfl_sync(0xffffffffu, l[x], 8 * t + 4 * e);
-          if (r >= a.rows) continue;
-          if (pc.whole) {
-            T* op = reinterpret_cast<T*>(a.o) + (int64_t)pc.b * a.o_b +
-                    (int64_t)(pc.head * a.group + r % a.group) * a.o_h + (int64_t)(r / a.group) * a.o_s + 4 * VW * g;
-            ew::Vec<T, 2 * MT> y;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              y.v[2 * i] = cvt<T>(L == 0.f ? 0.f : o[x][i][e] * iv);
-              y.v[2 * i + 1] = cvt<T>(L == 0.f ? 0.f : o[x][i][2 + e] * iv);
-            }
-            if (o_vec) {
-#pragma unroll
-              for (int i = 0; i < 2 * MT; i += 8)
-                *reinterpret_cast<uint4*>(op + i) = *reinterpret_cast<const uint4*>(&y.v[i]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 2 * MT; ++i) op[i] = y.v[i];
-            }
-          } else {
-            float* part = a.part + (int64_t)pc.slot * slot_floats(a.tile, D) + rt * D + 4 * VW * g;
-#pragma unroll
-            for (int i = 0; i < MT; i += 2)
-              *reinterpret_cast<float4*>(part + 2 * i) =
-                  make_float4(o[x][i][e], o[x][i][2 + e], o[x][i + 1][e], o[x][i + 1][2 + e]);
-          }
-        }
-        if (!pc.whole && t == 0) {
-          float* part = a.part + (int64_t)pc.slot * slot_floats(a.tile, D) + (int64_t)a.tile * D + 2 * (8 * x + g);
-          part[0] = m[x];
-          part[1] = l[x];
+        for (int i = 0; i < E / 4; ++i) {
+          const float4 y = *reinterpret_cast<const float4*>(slot + (w * 8 + rr) * D + (((c0 + i) ^ rr) << 2));
+          acc[4 * i] = fmaf(y.x, f, acc[4 * i]);
+          acc[4 * i + 1] = fmaf(y.y, f, acc[4 * i + 1]);
+          acc[4 * i + 2] = fmaf(y.z, f, acc[4 * i + 2]);
+          acc[4 * i + 3] = fmaf(y.w, f, acc[4 * i + 3]);
         }
       }
+      if (!ok || r >= a.rows) continue;
+      if (pc.whole) {
+        T* op = reinterpret_cast<T*>(a.o) + (int64_t)pc.b * a.o_b + (int64_t)(pc.head * a.group + r % a.group) * a.o_h +
+                (int64_t)(r / a.group) * a.o_s + 4 * c0;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        ew::Vec<T, E> y;
+#pragma unroll
+        for (int i = 0; i < E; ++i) y.v[i] = cvt<T>(L == 0.f ? 0.f : acc[i] * inv);
+        if (o_vec) {
+          *reinterpret_cast<ew::Vec<T, E>*>(op) = y;
+        } else {
+#pragma unroll
+          for (int i = 0; i < E; ++i) op[i] = y.v[i];
+        }
+      } else {
+        float* part = a.part + (int64_t)pc.slot * slot_floats(a.tile, D);
+#pragma unroll
+        for (int i = 0; i < E; i += 4)
+          *reinterpret_cast<float4*>(part + rt * D + 4 * c0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+        if (c0 == 0) *reinterpret_cast<float2*>(part + a.tile * D + 2 * rt) = make_float2(M, L);
+      }
     }
+    // the slot goes back to the copies: ordinary accesses before them are done
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    consumer_sync();
+    if (lane == 0) sm100::mbar_arrive(&v_empty[last]);
   }
 }
 

@@ -220,19 +220,30 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
           ok = sm100::mbar_wait(v ? &v_empty[st] : &k_empty[st], phase, abort_flag, a.err);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
-        if (v == 0 && lane < 16) {  // 16-byte records {ks, vs, id, -}, read with K
-          float* rec = reinterpret_cast<float*>(dyn + C::REC + st * 128) + grp * 4;
-          rec[is_v ? 1 : 0] = sc0;
-          if (!is_v) reinterpret_cast<int*>(rec)[2] = id0;
-        }
         const bool mine = first && is_v == (v == 1) && id0 >= 0;
-        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine));
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive_expect_tx(full, boxes * (uint32_t)(box * D));
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * (uint32_t)(box * D);
+        // K's one arrival follows the scales, whose load may still be under way; the copies' bytes
+        // are announced before the first can land.
+        if (lane == 0) {
+          if (v) sm100::mbar_arrive_expect_tx(full, bytes);
+          else
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(sm100::smem_u32(full)),
+                         "r"(bytes)
+                         : "memory");
+        }
         __syncwarp();
         if (mine)
           sm100::tma_load_4d(dyn + st * C::STAGE + (v ? C::K_BYTES : 0) + 16 * grp * D, v ? &tv : &tk, full, 0, in_page,
                              w0.head, id0);
+        if (v == 0) {
+          if (lane < 16) {  // 16-byte records {ks, vs, id, -}, read with K
+            float* rec = reinterpret_cast<float*>(dyn + C::REC + st * 128) + grp * 4;
+            rec[is_v ? 1 : 0] = sc0;
+            if (!is_v) reinterpret_cast<int*>(rec)[2] = id0;
+          }
+          __syncwarp();
+          if (lane == 0) sm100::mbar_arrive(full);
+        }
         ++armed;
       }
       if (!ok) break;
@@ -553,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
     // the slot goes back to the copies: ordinary accesses before them are done
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     consumer_sync();
-    if (lane == 0) sm100::mbar_arrive(&v_empty[last]);
+    if (lane == 0 && ok) sm100::mbar_arrive(&v_empty[last]);
   }
 }
 

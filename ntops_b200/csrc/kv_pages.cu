@@ -148,6 +148,11 @@ __device__ __forceinline__ int block_scan(int v, int* total) {
   return (warp ? part[warp - 1] : 0) + x - v;
 }
 
+// What one block may do by itself: tables and pools of up to this many entries (a few microseconds).
+// Larger ones take a launch with a block for each row first; the crossing is flat (64 rows of 32
+// pages: one launch less, 4 us of the host's time).
+constexpr int64_t kOneBlock = 1 << 15;
+
 // Gives the lowest free pages (refs 0) to the requests 0 .. wanted - 1 in their order: take(k, p)
 // for request k and page p, whose refs become 1.  Returns how many requests got a page.
 template <typename Take>
@@ -160,7 +165,7 @@ __device__ __forceinline__ int assign_free(int* refs, int P, int wanted, Take ta
     int n = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      f[e] = p + e < P && refs[p + e] == 0;
+      f[e] = p + e < P && __ldcg(refs + p + e) == 0;  // (atomics changed them in L2)
       n += f[e];
     }
     int total;
@@ -184,6 +189,7 @@ struct ExtendArgs {
   int* out;            // [B, M] contiguous
   const int* lengths;
   int64_t len_s;
+  const int* old_refs;
   int* refs;           // a copy of the caller's, updated
   int P, T;
   int* missing;
@@ -193,23 +199,33 @@ struct ExtendArgs {
 // Copies the table and lists, in row order, the entries that a row's length covers but that hold
 // no page; then hands out pages.  One block: a table is some ten thousand entries.
 __global__ void __launch_bounds__(kPlanThreads) extend_kernel(ExtendArgs a) {
-  const int64_t n = (int64_t)a.in.B * a.in.M;
+  const int n = a.in.B * a.in.M;
+  constexpr int E = 4;  // entries of a thread at a time
   int wanted = 0;
-  for (int64_t i0 = 0; i0 < n; i0 += kPlanThreads) {
-    const int64_t i = i0 + threadIdx.x;
-    int need = 0;
-    if (i < n) {
-      const int b = (int)(i / a.in.M), m = (int)(i % a.in.M);
-      const int id = page_of(a.in, a.P, b, m);
-      need = id < 0 && (int64_t)m * a.T < a.lengths[(int64_t)b * a.len_s];
-      a.out[i] = id;
+  for (int p = threadIdx.x; p < a.P; p += kPlanThreads) a.refs[p] = a.old_refs[p];
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads * E) {
+    const int i = i0 + (int)threadIdx.x * E;
+    bool need[E];
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      need[e] = false;
+      if (i + e < n) {
+        const int b = (i + e) / a.in.M, m = (i + e) - b * a.in.M;
+        const int id = page_of(a.in, a.P, b, m);
+        need[e] = id < 0 && (int64_t)m * a.T < a.lengths[(int64_t)b * a.len_s];
+        a.out[i + e] = id;
+      }
+      c += need[e];
     }
     int total;
-    const int k = wanted + block_scan(need, &total);
-    if (need) a.want[k] = (int)i;
+    int k = wanted + block_scan(c, &total);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (need[e]) a.want[k++] = i + e;
     wanted += total;
   }
-  __syncthreads();  // want[] is written
+  __syncthreads();  // want[] and refs[] are written
   const int got = assign_free(a.refs, a.P, wanted, [&](int k, int p) { a.out[a.want[k]] = p; });
   if (threadIdx.x == 0) *a.missing = wanted - got;
 }
@@ -220,46 +236,32 @@ struct ReorderArgs {
   const int *lengths, *parents;
   int64_t len_s, par_s;
   int* new_lengths;            // [N]
+  const int* old_refs;
   int* refs;                   // a copy of the caller's, updated
   int N, P, T;
   int* missing;
   int *need, *want, *src, *dst, *count;  // workspace: [N] each, and one
 };
 
-// One block a row.  Blocks of old rows take their references away; blocks of new rows write the
-// row, add its references and note the page it needs its own copy of.
-__global__ void __launch_bounds__(128) reorder_rows_kernel(ReorderArgs a) {
-  const int M = a.in.M;
-  if ((int)blockIdx.x < a.in.B) {
-    for (int m = threadIdx.x; m < M; m += blockDim.x) {
-      const int id = page_of(a.in, a.P, blockIdx.x, m);
-      if (id >= 0) atomicSub(&a.refs[id], 1);
-    }
+// New row i, by the threads that call it together (tid of n): the row, its references, and the page
+// it needs its own copy of.  `earlier`: an earlier new row continues the same old one.
+__device__ __forceinline__ void new_row(const ReorderArgs& a, int i, bool earlier, int tid, int n) {
+  const int M = a.in.M, p = a.parents[(int64_t)i * a.par_s];
+  const bool ok = (unsigned)p < (unsigned)a.in.B;
+  const int len = ok ? max(a.lengths[(int64_t)p * a.len_s], 0) : 0;
+  const int whole = len / a.T, part = len % a.T;
+  if (tid == 0) {
+    a.new_lengths[i] = len;
+    a.need[i] = ok && earlier && part ? page_of(a.in, a.P, p, whole) : -1;
   }
-  if ((int)blockIdx.x < a.N) {
-    const int i = blockIdx.x;
-    const int p = a.parents[(int64_t)i * a.par_s];
-    const bool ok = (unsigned)p < (unsigned)a.in.B;
-    int earlier = 0;  // does an earlier new row continue the same old row?
-    for (int j = threadIdx.x; j < i; j += blockDim.x) earlier |= a.parents[(int64_t)j * a.par_s] == p;
-    const bool first = !__syncthreads_or(earlier);
-    const int len = ok ? max(a.lengths[(int64_t)p * a.len_s], 0) : 0;
-    const int whole = len / a.T, part = len % a.T;
-    if (threadIdx.x == 0) {
-      a.new_lengths[i] = len;
-      a.need[i] = ok && !first && part ? page_of(a.in, a.P, p, whole) : -1;
-    }
-    for (int m = threadIdx.x; m < M; m += blockDim.x) {
-      const int id = ok && (first || m < whole) ? page_of(a.in, a.P, p, m) : -1;
-      a.out[(int64_t)i * M + m] = id;
-      if (id >= 0) atomicAdd(&a.refs[id], 1);
-    }
+  for (int m = tid; m < M; m += n) {
+    const int id = ok && (!earlier || m < whole) ? page_of(a.in, a.P, p, m) : -1;
+    a.out[(int64_t)i * M + m] = id;
+    if (id >= 0) atomicAdd(&a.refs[id], 1);
   }
 }
-
 // Hands pages to the new rows that need a copy, in row order, and lists the copies.
-__global__ void __launch_bounds__(kPlanThreads) reorder_assign_kernel(ReorderArgs a) {
-  grid_dependency_wait();
+__device__ __forceinline__ void assign_copies(const ReorderArgs& a) {
   int wanted = 0;
   for (int i0 = 0; i0 < a.N; i0 += kPlanThreads) {
     const int i = i0 + threadIdx.x;
@@ -282,6 +284,47 @@ __global__ void __launch_bounds__(kPlanThreads) reorder_assign_kernel(ReorderArg
   }
 }
 
+// Everything but the copies in one block.
+__global__ void __launch_bounds__(kPlanThreads) reorder_plan_kernel(ReorderArgs a) {
+  grid_dependency_launch();
+  for (int p = threadIdx.x; p < a.P; p += kPlanThreads) a.refs[p] = a.old_refs[p];
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.in.B * a.in.M; i += kPlanThreads) {
+    const int id = page_of(a.in, a.P, i / a.in.M, i % a.in.M);
+    if (id >= 0) atomicSub(&a.refs[id], 1);
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = warp; i < a.N; i += kPlanThreads / 32) {
+    const int p = a.parents[(int64_t)i * a.par_s];
+    int earlier = 0;
+    for (int j = lane; j < i; j += 32) earlier |= a.parents[(int64_t)j * a.par_s] == p;
+    new_row(a, i, __any_sync(0xffffffffu, earlier), lane, 32);
+  }
+  __syncthreads();
+  assign_copies(a);
+}
+
+// The same in two launches, the first with one block a row: blocks of old rows take their
+// references away, blocks of new rows write the rows.
+__global__ void __launch_bounds__(128) reorder_rows_kernel(ReorderArgs a) {
+  if ((int)blockIdx.x < a.in.B) {
+    for (int m = threadIdx.x; m < a.in.M; m += blockDim.x) {
+      const int id = page_of(a.in, a.P, blockIdx.x, m);
+      if (id >= 0) atomicSub(&a.refs[id], 1);
+    }
+  }
+  if ((int)blockIdx.x < a.N) {
+    const int i = blockIdx.x, p = a.parents[(int64_t)i * a.par_s];
+    int earlier = 0;
+    for (int j = threadIdx.x; j < i; j += blockDim.x) earlier |= a.parents[(int64_t)j * a.par_s] == p;
+    new_row(a, i, __syncthreads_or(earlier), threadIdx.x, blockDim.x);
+  }
+}
+__global__ void __launch_bounds__(kPlanThreads) reorder_assign_kernel(ReorderArgs a) {
+  grid_dependency_wait();
+  assign_copies(a);
+}
+
 struct CompactArgs {
   Table in;
   int* out;
@@ -291,11 +334,13 @@ struct CompactArgs {
   int* used;
   int P;
   int *map, *src, *dst, *count;  // workspace: [P] each, and one
+  int one_block;               // the plan's block maps the table too
 };
 
 // Counts the used pages U, lists the used pages past the first U and the free pages among them,
 // both in ascending order: the k-th of the one moves to the k-th of the other.
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs a) {
+  grid_dependency_launch();
   int n = 0, U, total;
   for (int p = threadIdx.x; p < a.P; p += kPlanThreads) n += a.refs[(int64_t)p * a.ref_s] > 0;
   block_scan(n, &U);
@@ -324,6 +369,13 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs 
     *a.count = movers;
     *a.used = U;
   }
+  if (a.one_block) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.in.B * a.in.M; i += kPlanThreads) {
+      const int id = page_of(a.in, a.P, i / a.in.M, i % a.in.M);
+      a.out[i] = id < 0 ? -1 : a.map[id];
+    }
+  }
 }
 
 __global__ void __launch_bounds__(256) compact_table_kernel(CompactArgs a) {
@@ -349,13 +401,6 @@ int check_out(const NtbTensor* t, int ndim, const char* name) {
   int rc = check_i32(t, ndim, name);
   if (rc != NTB_OK) return rc;
   NTB_ARG(is_contiguous(t), "%s must be contiguous", name);
-  return NTB_OK;
-}
-
-// refs_out = refs, on the stream.
-int copy_refs(const NtbTensor* refs, const NtbTensor* out, cudaStream_t st) {
-  if (numel(refs) == 0) return NTB_OK;
-  NTB_CUDA(cudaMemcpyAsync(out->data, refs->data, (size_t)numel(refs) * 4, cudaMemcpyDeviceToDevice, st));
   return NTB_OK;
 }
 
@@ -410,10 +455,10 @@ extern "C" int ntb_kv_extend(const NtbTensor* block_table, const NtbTensor* leng
   NTB_ARG(workspace_bytes >= need && (workspace != nullptr || need == 0), "workspace too small: %lld bytes, need %lld",
           (long long)workspace_bytes, (long long)need);
   cudaStream_t st = (cudaStream_t)stream;
-  if ((rc = copy_refs(refs, refs_out, st)) != NTB_OK) return rc;
   a.out = reinterpret_cast<int*>(table_out->data);
   a.lengths = reinterpret_cast<const int*>(lengths->data);
   a.len_s = lengths->stride[0];
+  a.old_refs = reinterpret_cast<const int*>(refs->data);
   a.refs = reinterpret_cast<int*>(refs_out->data);
   a.P = (int)refs->shape[0];
   a.T = (int)page_size;
@@ -457,7 +502,6 @@ extern "C" int ntb_kv_reorder(const NtbKvCache* cache, const NtbTensor* block_ta
   NTB_ARG(workspace != nullptr && workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
           (long long)workspace_bytes, (long long)need);
   cudaStream_t st = (cudaStream_t)stream;
-  if ((rc = copy_refs(refs, refs_out, st)) != NTB_OK) return rc;
   int* ws = reinterpret_cast<int*>(workspace);
   a.out = reinterpret_cast<int*>(table_out->data);
   a.lengths = reinterpret_cast<const int*>(lengths->data);
@@ -465,6 +509,7 @@ extern "C" int ntb_kv_reorder(const NtbKvCache* cache, const NtbTensor* block_ta
   a.len_s = lengths->stride[0];
   a.par_s = parents->stride[0];
   a.new_lengths = reinterpret_cast<int*>(lengths_out->data);
+  a.old_refs = reinterpret_cast<const int*>(refs->data);
   a.refs = reinterpret_cast<int*>(refs_out->data);
   a.N = (int)N;
   a.P = c.P;
@@ -476,11 +521,17 @@ extern "C" int ntb_kv_reorder(const NtbKvCache* cache, const NtbTensor* block_ta
   a.src = a.want + N;
   a.dst = a.src + N;
   const int rows = std::max(a.in.B, a.N);
-  if (rows > 0) {
+  // (the pairwise look at the parents grows with N * N)
+  if (((int64_t)a.in.B + N) * std::max(a.in.M, 1) + a.P + N * N / 32 <= kOneBlock) {
+    reorder_plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
+    NTB_LAUNCH_CHECK();
+  } else {
+    if (a.P > 0)
+      NTB_CUDA(cudaMemcpyAsync(refs_out->data, refs->data, (size_t)a.P * 4, cudaMemcpyDeviceToDevice, st));
     reorder_rows_kernel<<<rows, 128, 0, st>>>(a);
     NTB_LAUNCH_CHECK();
+    NTB_CUDA(launch_dependent(reorder_assign_kernel, dim3(1), dim3(kPlanThreads), 0, st, a));
   }
-  NTB_CUDA(launch_dependent(reorder_assign_kernel, dim3(1), dim3(kPlanThreads), 0, st, a));
   c.src = a.src;
   c.dst = a.dst;
   c.src_s = c.dst_s = 1;
@@ -523,10 +574,11 @@ extern "C" int ntb_kv_compact(const NtbKvCache* cache, const NtbTensor* block_ta
   a.map = ws + 1;
   a.src = a.map + c.P;
   a.dst = a.src + c.P;
+  const int64_t n = numel(block_table);
+  a.one_block = n <= kOneBlock;
   compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
   NTB_LAUNCH_CHECK();
-  const int64_t n = numel(block_table);
-  if (n > 0) {
+  if (n > 0 && !a.one_block) {
     const int64_t grid = std::min<int64_t>((n + 255) / 256, 4ll * sm_count());
     NTB_CUDA(launch_dependent(compact_table_kernel, dim3((unsigned)grid), dim3(256), 0, st, a));
   }

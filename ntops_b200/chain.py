@@ -10,6 +10,10 @@ Layouts are chosen so no operator needs a copy: projections produce [B*S, H*D] r
 viewed as [B, S, H, D] for RoPE and as [B, H, S, D] (a transposed view) for attention, whose
 output keeps the query's memory layout (as the reference's ``torch.empty_like(query)`` does),
 so the output projection reads it back as [B*S, H*D] rows.
+
+``layer_step`` is the same layer in serving: it takes the next tokens of a batch of sequences
+(whole prompts, chunks of them or single tokens), stores their keys and values in a paged 8-bit
+cache (``ntops_b200.kv_cache``) and attends over it.
 """
 
 import torch
@@ -141,3 +145,34 @@ def layer_forward(x, wts, sin, cos, mm_hook=None, fused=True):
         act = nt.mul(nt.silu(gate), up)
     down = mm(act, wts.wd)
     return down.view(B, S, HIDDEN)
+
+
+def layer_step(x, wts, sin, cos, cache_layer, block_table, start, lengths):
+    """The layer on the next tokens x [B, S, 4096] (bf16) of B sequences, over a layer of a paged 8-bit
+    KV cache; returns [B, S, 4096].
+
+    Row b's tokens stand at positions start[b] .. start[b] + S - 1, its cache holds lengths[b] tokens
+    once they are stored (start, lengths: int32 [B] on the device; for a ragged prompt chunk
+    lengths[b] - start[b] may be less than S, and the rows past it are to be ignored).  sin / cos:
+    tables for every position the cache can hold.  Pages for the new tokens must be in the table
+    (``kv_cache.extend``)."""
+    from ntops_b200 import fused as F
+    from ntops_b200 import kv_cache
+
+    B, S, _ = x.shape
+    T = B * S
+    x2 = x.reshape(T, HIDDEN)
+    h = nt.rms_norm(x2, (HIDDEN,), wts.norm1, EPS)
+    # each row's own positions: the rotation sees one sequence of B * S rows with gathered tables
+    pos = (start.view(B, 1) + torch.arange(S, device=x.device)).clamp(0, sin.shape[0] - 1).view(T).long()
+    sin_r, cos_r = sin[pos], cos[pos]
+    q = nt.mm(h, wts.wq).view(1, T, HEADS, HEAD_DIM)
+    k = nt.mm(h, wts.wk).view(1, T, KV_HEADS, HEAD_DIM)
+    v = nt.mm(h, wts.wv).view(B, S, KV_HEADS, HEAD_DIM)
+    q = nt.rotary_position_embedding(q, sin_r, cos_r, interleaved=False, inplace=True).view(B, S, HEADS, HEAD_DIM)
+    k = nt.rotary_position_embedding(k, sin_r, cos_r, interleaved=False, inplace=True).view(B, S, KV_HEADS, HEAD_DIM)
+    kv_cache.store(cache_layer, k.transpose(1, 2), v.transpose(1, 2), block_table, start, counts=lengths - start)
+    o = kv_cache.attention(q.transpose(1, 2), cache_layer, block_table, lengths, start=start)
+    attn = nt.mm(o.transpose(1, 2).reshape(T, HEADS * HEAD_DIM), wts.wo)
+    x2, h2 = F.add_rms_norm(x2, attn, wts.norm2, EPS)
+    return nt.mm(F.swiglu_linear(h2, wts.wgu), wts.wd).view(B, S, HIDDEN)

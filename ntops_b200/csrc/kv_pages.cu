@@ -37,23 +37,30 @@ constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 4;
 constexpr int kCopyChunk = kCopyThreads * kCopyUnroll * 16;  // bytes of a work item
 
+// Work items are (pair, layer, key or value, chunk), chunks fastest.  The next item's page numbers
+// are loaded while this one's bytes move.
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(CopyArgs a) {
   grid_dependency_wait();
   const int pairs = a.count == nullptr ? a.pairs : min(max(*a.count, 0), a.pairs);
   const int chunks = (int)((a.block + kCopyChunk - 1) / kCopyChunk);
-  const int64_t items = (int64_t)pairs * a.L * 2 * chunks;
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    int64_t r = it;
-    const int c = (int)(r % chunks);
-    r /= chunks;
-    const int w = (int)(r & 1);
-    r >>= 1;
-    const int l = (int)(r % a.L);
-    const int64_t k = r / a.L;
-    const int src = a.src[k * a.src_s], dst = a.dst[k * a.dst_s];
-    if ((unsigned)src >= (unsigned)a.P || (unsigned)dst >= (unsigned)a.P || src == dst) continue;
-    const uint8_t* s = a.code[w] + (int64_t)l * a.c_l[w] + (int64_t)src * a.c_p[w];
-    uint8_t* d = a.code[w] + (int64_t)l * a.c_l[w] + (int64_t)dst * a.c_p[w];
+  const int per_pair = a.L * 2 * chunks;  // (the host checks that all items fit 31 bits)
+  const int items = pairs * per_pair;
+  int src = -1, dst = -1;
+  if ((int)blockIdx.x < items) {
+    src = a.src[(int)blockIdx.x / per_pair * a.src_s];
+    dst = a.dst[(int)blockIdx.x / per_pair * a.dst_s];
+  }
+  for (int it = blockIdx.x; it < items; it += gridDim.x) {
+    const int r = it % per_pair, c = r % chunks, w = (r / chunks) & 1, l = r / chunks >> 1;
+    const int from = src, to = dst;
+    if (it + (int)gridDim.x < items) {
+      const int64_t k = (it + (int)gridDim.x) / per_pair;
+      src = a.src[k * a.src_s];
+      dst = a.dst[k * a.dst_s];
+    }
+    if ((unsigned)from >= (unsigned)a.P || (unsigned)to >= (unsigned)a.P || from == to) continue;
+    const uint8_t* s = a.code[w] + (int64_t)l * a.c_l[w] + (int64_t)from * a.c_p[w];
+    uint8_t* d = a.code[w] + (int64_t)l * a.c_l[w] + (int64_t)to * a.c_p[w];
     const int64_t lo = (int64_t)c * kCopyChunk, hi = min(a.block, lo + kCopyChunk);
     if (a.dense) {
       uint4 v[kCopyUnroll];
@@ -77,7 +84,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(CopyArgs a) {
     if (c == 0)
       for (int h = threadIdx.x; h < a.H; h += kCopyThreads) {
         float* sc = a.scale[w] + (int64_t)l * a.s_l[w] + (int64_t)h * a.s_h[w];
-        sc[(int64_t)dst * a.s_p[w]] = sc[(int64_t)src * a.s_p[w]];
+        sc[(int64_t)to * a.s_p[w]] = sc[(int64_t)from * a.s_p[w]];
       }
   }
 }
@@ -113,6 +120,7 @@ int launch_copy(const CopyArgs& a, cudaStream_t st) {
   const int64_t chunks = (a.block + kCopyChunk - 1) / kCopyChunk;
   const int64_t most = (int64_t)a.pairs * a.L * 2 * chunks;
   if (most == 0) return NTB_OK;
+  NTB_UNSUP(most <= 0x3fffffffLL, "too many bytes to copy in one call");
   const int64_t grid = std::min<int64_t>(most, resident_blocks((const void*)copy_kernel, kCopyThreads, 0));
   NTB_CUDA(launch_dependent(copy_kernel, dim3((unsigned)grid), dim3(kCopyThreads), 0, st, a));
   return NTB_OK;

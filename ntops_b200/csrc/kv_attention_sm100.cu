@@ -5,10 +5,12 @@
 // block serves the whole group) and walks its keys in blocks of 128:
 //   warp 1      looks up pages and scales and copies the codes of half a block (64 keys) of K or V
 //               at a time into staging slots with TMA;
-//   warps 4-7   widen codes to fp16 (exact) into the swizzled operand tiles, two of K and two of V;
-//   warp 0      issues S_t = Q_t K^T (both from shared memory) and O_t += P_t V (P from TMEM) in the
-//               order PV_0(j), S_0(j+1), PV_1(j), S_1(j+1): one tile's products run during the
-//               other's softmax;
+//   warps 4-7   widen codes to fp16 (exact) into the swizzled operand tiles, two of K (warps 4, 5) and
+//               two of V (6, 7);
+//   warps 0, 2  issue the products of tile 0 and of tile 1 for half blocks (64 keys) i: S_t(i) = Q_t
+//               K^T (both from shared memory) and O_t += P_t(i) V (P from TMEM), in the order PV_t(i),
+//               S_t(i+2).  A tile's scores have two TMEM buffers, so the next half block's are there
+//               while its softmax still works on this one's;
 //   warps 8-15  one thread a row: load Q (multiplied by a power of two that puts the row's largest
 //               element in [2^14, 2^15), so fp16 holds it as exactly as the input type), take S from
 //               TMEM, keep the running maximum, write P = exp2(.) in fp16 over S.
@@ -21,7 +23,7 @@
 // cycles, the products' time as well).  Where one wave of blocks would leave SMs idle, several
 // blocks share a tile's keys and kv_split_combine joins them.
 #include <algorithm>
-#include <atomic>
+#include <type_traits>
 
 #include "kv_attention.cuh"
 #include "sm100.cuh"
@@ -34,15 +36,12 @@ namespace {
 constexpr int BLK = 128;
 constexpr int kTiles = 2;
 constexpr int kThreads = 512;
-constexpr int kMmaWarp = 0, kTmaWarp = 1, kConvBase = 4, kSoftBase = 8;
-// Register split (setmaxnreg) of 512 threads launched with 128 each: the sum over the warpgroups
-// must not exceed the launch's, or the raise would wait forever; the host checks the latter.
-constexpr int kLaunchRegs = 128, kProdRegs = 56, kConvRegs = 72, kSoftRegs = 192;
-static_assert(kProdRegs + kConvRegs + 2 * kSoftRegs <= 4 * kLaunchRegs, "register split too large");
+constexpr int kMmaWarp = 0, kTmaWarp = 1, kConvBase = 4, kSoftBase = 8;  // warps 0 and 2 issue tiles 0 and 1
 constexpr float kRescaleThreshold = 8.f;
 constexpr int kHalf = 64;       // keys of a staging slot
 constexpr int kInfo = 4;        // blocks whose scales are kept: see info_full below
-constexpr uint32_t kSCol = 0, kOCol = 256;  // TMEM columns: S_t at 128 t (P_t over its first 64), O_t at 256 + 128 t
+// TMEM columns: S_t's buffer b at 128 t + 64 b (P over its first 32), O_t at 256 + 128 t.
+constexpr uint32_t kSCol = 0, kOCol = 256;
 
 template <int D>
 struct Smem {
@@ -57,7 +56,7 @@ struct Smem {
   static constexpr int SV = SK + 2 * SLOT;
   static constexpr int INFO = SV + 2 * SLOT;     // kInfo x 80 bytes
   static constexpr int BAR = INFO + 512;
-  static constexpr int TOTAL = BAR + 256 + 1024;
+  static constexpr int TOTAL = BAR + 320 + 1024;
   static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -114,6 +113,11 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint32_t x, uint32_t y, uin
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// tcgen05.mma with A in TMEM, the accumulate flag at run time.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, bool acc) {
+  sm100::mma_f16_ts(d, a, (uint64_t)b_lo | ((uint64_t)b_hi << 32), idesc, acc ? 1u : 0u);
+}
+
 // True in one lane of a converged warp, always the same one.  Under a test of the lane number the
 // compiler has to move every descriptor half from a thread's to a uniform register for each
 // instruction (about 64 cycles a tcgen05.mma, measured, whatever its size); under this one the
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::BAR);
-  uint64_t* q_full = bars + 0;
+  uint64_t* q_full = bars + 33;   // [tile]
   uint64_t* k_full = bars + 1;    // [2] fp16 tiles
   uint64_t* k_empty = bars + 3;   // [2]
   uint64_t* v_full = bars + 5;    // [2]
@@ -175,15 +179,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* sk_empty = bars + 11; // [2]
   uint64_t* sv_full = bars + 13;  // [2]
   uint64_t* sv_empty = bars + 15; // [2]
-  uint64_t* s_full = bars + 17;   // [tile]
-  uint64_t* p_full = bars + 19;   // [tile]
-  uint64_t* pv_done = bars + 21;  // [tile]
+  uint64_t* s_full = bars + 17;   // [tile][buffer]
+  uint64_t* p_full = bars + 21;   // [tile][buffer]
+  uint64_t* pv_done = bars + 25;  // [tile]
   // [kInfo] scales of block j.  The producer writes entry j once the converters are through K(j - 1)'s
-  // first slot: they had its tile, so K(j - 3)'s products were done, and those of the second row tile
-  // were issued after both tiles' P(j - 4): entry j - 4 is no longer read.
-  uint64_t* info_full = bars + 23;
-  uint64_t* done_bar = bars + 27;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
+  // first slot, so they had its tile, so K(j - 3)'s products were done; those of its last half block
+  // were issued after both tiles' P of block j - 4: entry j - 4 is no longer read.
+  uint64_t* info_full = bars + 27;
+  uint64_t* done_bar = bars + 31;  // [tile]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 35);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Info* info = reinterpret_cast<Info*>(sm + S::INFO);
 
@@ -213,22 +217,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   if (threadIdx.x == 0) {
-    sm100::mbar_init(q_full, 256);
+    const uint32_t users = (n_t[0] > 0) + (n_t[1] > 0);  // tiles that release a block's K and V
     for (int i = 0; i < 2; ++i) {
+      sm100::mbar_init(&q_full[i], 128);
+      sm100::mbar_init(&done_bar[i], 1);
       sm100::mbar_init(&k_full[i], 64);
-      sm100::mbar_init(&k_empty[i], 1);
+      sm100::mbar_init(&k_empty[i], max(users, 1u));
       sm100::mbar_init(&v_full[i], 64);
-      sm100::mbar_init(&v_empty[i], 1);
+      sm100::mbar_init(&v_empty[i], max(users, 1u));
       sm100::mbar_init(&sk_full[i], 1);
       sm100::mbar_init(&sk_empty[i], 2);
       sm100::mbar_init(&sv_full[i], 1);
       sm100::mbar_init(&sv_empty[i], 2);
-      sm100::mbar_init(&s_full[i], 1);
-      sm100::mbar_init(&p_full[i], 128);
       sm100::mbar_init(&pv_done[i], 1);
     }
+    for (int i = 0; i < 4; ++i) {
+      sm100::mbar_init(&s_full[i], 1);
+      sm100::mbar_init(&p_full[i], 128);
+    }
     for (int i = 0; i < kInfo; ++i) sm100::mbar_init(&info_full[i], 1);
-    sm100::mbar_init(done_bar, 1);
     *abort_flag = 0;
     sm100::fence_mbar_init();
   }
@@ -243,7 +250,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_dependency_launch();
 
   if (warp < kConvBase) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProdRegs));
     if (warp == kTmaWarp) {
       // --------------------------------------------------------------- producer ----
       // lanes 0-7: the block's 8 groups of 16 keys of K; lanes 8-15: of V.  The lane of a box's
@@ -323,81 +329,82 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (uses > 0) sm100::mbar_wait_unwind(q >= 2 ? &sv_full[q & 1] : &sk_full[q & 1], (uint32_t)((uses - 1) & 1));
         }
       __syncwarp();
-    } else if (warp == kMmaWarp) {
-      // ------------------------------------------------------------- MMA issuer ----
-      constexpr uint32_t idesc_qk = sm100::instr_desc(0, false, false, BLK, BLK);
+    } else if (warp == kMmaWarp || warp == kMmaWarp + 2) {
+      // ------------------------------------------------------------ MMA issuers ----
+      constexpr uint32_t idesc_qk = sm100::instr_desc(0, false, false, BLK, kHalf);
       constexpr uint32_t idesc_pv = sm100::instr_desc(0, false, true, BLK, D);
-      bool ok = n > 0 && sm100::mbar_wait(q_full, 0, abort_flag, a.err);
+      const int t = warp >> 1, h = 2 * n_t[t];  // half blocks of this tile
+      bool ok = h > 0 && sm100::mbar_wait(&q_full[t], 0, abort_flag, a.err);
       sm100::tc_fence_after();
       const uint32_t d_hi = sm100::smem_desc_hi(1024);
-      const uint32_t q_lo = sm100::smem_desc_lo(sm100::smem_u32(sm + S::Q), 16);
+      // low descriptor halves; a tile further is TILE bytes in the address field
+      constexpr uint32_t kTileStep = S::TILE >> 4, kHalfStep = kHalf * 128 >> 4;
+      const uint32_t q_lo = sm100::smem_desc_lo(sm100::smem_u32(sm + S::Q), 16) + t * kTileStep;
       const uint32_t k_lo = sm100::smem_desc_lo(sm100::smem_u32(sm + S::K), 16);
       const uint32_t v_lo = sm100::smem_desc_lo(sm100::smem_u32(sm + S::V), S::SUB);
-      constexpr uint32_t kTileStep = S::TILE >> 4;
-      // S_t(j) = Q_t K_j^T; K_j's first user waits for it, its last one releases it.
-      auto issue_s = [&](int t, int j) -> bool {
-        const int st = j & 1;
-        if (t == 0 || j >= n_t[0]) {
-          if (!sm100::mbar_wait(&k_full[st], (uint32_t)((j >> 1) & 1), abort_flag, a.err)) return false;
+      const uint32_t s_col = tmem + kSCol + 128u * t, o_col = tmem + kOCol + 128u * t;
+      // S_t(i) = Q_t K^T of half block i; the block's second half releases K.
+      auto issue_s = [&](int i) -> bool {
+        const int st = (i >> 1) & 1, b = i & 1;
+        if (b == 0) {
+          if (!sm100::mbar_wait(&k_full[st], (uint32_t)((i >> 2) & 1), abort_flag, a.err)) return false;
           sm100::tc_fence_after();
         }
         if (elect_one()) {
-          const uint32_t a0 = q_lo + t * kTileStep, b0 = k_lo + st * kTileStep, d = tmem + kSCol + 128u * t;
+          const uint32_t b0 = k_lo + st * kTileStep + b * kHalfStep, d = s_col + 64u * b;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = ((kk >> 2) * S::SUB + (kk & 3) * 32) >> 4;
-            if (kk == 0) sm100::mma_f16_lohi<false>(d, a0 + off, d_hi, b0 + off, d_hi, idesc_qk);
-            else sm100::mma_f16_lohi<true>(d, a0 + off, d_hi, b0 + off, d_hi, idesc_qk);
+            if (kk == 0) sm100::mma_f16_lohi<false>(d, q_lo + off, d_hi, b0 + off, d_hi, idesc_qk);
+            else sm100::mma_f16_lohi<true>(d, q_lo + off, d_hi, b0 + off, d_hi, idesc_qk);
           }
-          sm100::mma_commit(&s_full[t]);
-          if (t == 1 || j >= n_t[1]) sm100::mma_commit(&k_empty[st]);
+          sm100::mma_commit(&s_full[2 * t + b]);
+          if (b == 1) sm100::mma_commit(&k_empty[st]);
         }
         __syncwarp();
         return true;
       };
-      // O_t += P_t(j) V_j, likewise.
-      auto issue_pv = [&](int t, int j) -> bool {
-        const int st = j & 1;
-        if (!sm100::mbar_wait(&p_full[t], (uint32_t)(j & 1), abort_flag, a.err)) return false;
-        if ((t == 0 || j >= n_t[0]) &&
-            !sm100::mbar_wait(&v_full[st], (uint32_t)((j >> 1) & 1), abort_flag, a.err))
-          return false;
+      // O_t += P_t(i) V, likewise.
+      auto issue_pv = [&](int i) -> bool {
+        const int st = (i >> 1) & 1, b = i & 1;
+        if (b == 0 && !sm100::mbar_wait(&v_full[st], (uint32_t)((i >> 2) & 1), abort_flag, a.err)) return false;
+        if (!sm100::mbar_wait(&p_full[2 * t + b], (uint32_t)((i >> 1) & 1), abort_flag, a.err)) return false;
         sm100::tc_fence_after();
         if (elect_one()) {
-          const uint32_t b0 = v_lo + st * kTileStep, p = tmem + kSCol + 128u * t, d = tmem + kOCol + 128u * t;
+          const uint32_t b0 = v_lo + st * kTileStep + b * kHalfStep, p = s_col + 64u * b;
 #pragma unroll
-          for (int kk = 0; kk < BLK / 16; ++kk) {
+          for (int kk = 0; kk < kHalf / 16; ++kk) {
             const uint32_t off = (kk * 16 * 128) >> 4;
-            if (kk == 0) sm100::mma_f16_ts(d, p, (uint64_t)b0 | ((uint64_t)d_hi << 32), idesc_pv, j != 0);
-            else sm100::mma_f16_ts_lohi<true>(d, p + kk * 8, b0 + off, d_hi, idesc_pv);
+            if (kk == 0) mma_ts(o_col, p, b0, d_hi, idesc_pv, i != 0);
+            else sm100::mma_f16_ts_lohi<true>(o_col, p + kk * 8, b0 + off, d_hi, idesc_pv);
           }
           sm100::mma_commit(&pv_done[t]);
-          if (t == 1 || j >= n_t[1]) sm100::mma_commit(&v_empty[st]);
+          if (b == 1) sm100::mma_commit(&v_empty[st]);
         }
         __syncwarp();
         return true;
       };
-      if (ok && n_t[0] > 0) ok = issue_s(0, 0);
-      if (ok && n_t[1] > 0) ok = issue_s(1, 0);
-      for (int j = 0; ok && j < n; ++j) {
-        if (j < n_t[0]) {
-          ok = issue_pv(0, j);
-          if (ok && j + 1 < n_t[0]) ok = issue_s(0, j + 1);
-        }
-        if (ok && j < n_t[1]) {
-          ok = issue_pv(1, j);
-          if (ok && j + 1 < n_t[1]) ok = issue_s(1, j + 1);
-        }
+      for (int i = 0; ok && i < 2; ++i) ok = issue_s(i);
+      for (int i = 0; ok && i < h; ++i) {
+        ok = issue_pv(i);
+        if (ok && i + 2 < h) ok = issue_s(i + 2);
       }
-      if (elect_one()) {
-        sm100::mma_commit(done_bar);
-        sm100::mbar_wait_unwind(done_bar, 0);
+      if (elect_one()) sm100::mma_commit(&done_bar[t]);  // every product of this tile
+      __syncwarp();
+      // blocks that only the other tile still uses: this one has nothing to hold them for
+      for (int j = n_t[t]; ok && j < n; ++j) {
+        const int st = j & 1;
+        const uint32_t phase = (uint32_t)((j >> 1) & 1);
+        ok = sm100::mbar_wait(&k_full[st], phase, abort_flag, a.err);
+        if (ok && lane == 0) sm100::mbar_arrive(&k_empty[st]);
+        if (ok) ok = sm100::mbar_wait(&v_full[st], phase, abort_flag, a.err);
+        if (ok && lane == 0) sm100::mbar_arrive(&v_empty[st]);
       }
+      if (lane == 0) sm100::mbar_wait_unwind(&done_bar[t], 0);
       __syncwarp();
     }
   } else if (warp < kSoftBase) {
     // ----------------------------------------------------------------- widening ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
     // Warps 4 and 5 widen K, 6 and 7 V; each takes 32 keys, two groups of 16, of every half block.
     // A step is 8 keys x 4 vectors of 16 codes; the loads of a half block are in flight together.
     const bool is_v = warp >= kConvBase + 2;
@@ -473,13 +480,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------ softmax ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     const int t = (warp - kSoftBase) >> 2;
     const int wq = warp & 3;                          // TMEM lane quarter
     const int rt = t * BLK + wq * 32 + lane;          // row in the block's pair of tiles
     const int r = r0 + rt;
     const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
-    const uint32_t s_tmem = tmem + kSCol + 128u * t + lane_addr;
+    const uint32_t s_col = tmem + kSCol + 128u * t + lane_addr;
     const uint32_t o_tmem = tmem + kOCol + 128u * t + lane_addr;
     // this row's query, scaled, into its swizzled tile row
     float rowsc;
@@ -530,77 +536,84 @@ __global__ void __launch_bounds__(kThreads, 1)
         *reinterpret_cast<uint4*>(q + (i >> 3) * S::SUB + (((i & 7) ^ sw) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
       }
       fence_async_smem();
-      sm100::mbar_arrive(q_full);
+      sm100::mbar_arrive(&q_full[t]);
     }
-    const int mine = n_t[t];
+    const int mine = 2 * n_t[t];
     const int kmax = r < a.rows ? last_key(a, len, start, r / a.group) : -1;
-    float m_used = -INFINITY, l = 0.f, vref = 1.f;
+    float m_used = -INFINITY, l = 0.f, vref = 1.f, sc = 1.f;
+    uint32_t holes = 0;
     bool ok = true;
-    for (int j = 0; j < mine; ++j) {
-      const int k0 = (jb + j) * BLK;
-      if (!sm100::mbar_wait(&info_full[j % kInfo], (uint32_t)((j / kInfo) & 1), abort_flag, a.err)) { ok = false; break; }
-      const Info* I = &info[j % kInfo];
-      // positive even for a zero scale (or one that underflows): masked scores are -inf, and -inf * 0
-      // would be NaN
-      float sc = rowsc * I->kref;
-      if (sc < 1.17549435e-38f) sc = 1.17549435e-38f;
-      const float vfac = I->vfac;
-      const uint32_t holes = I->holes;
-      vref = I->vref;
-      if (!sm100::mbar_wait(&s_full[t], (uint32_t)(j & 1), abort_flag, a.err)) { ok = false; break; }
+    for (int i = 0; i < mine; ++i) {
+      const int j = i >> 1, b = i & 1, k0 = (jb + j) * BLK + kHalf * b;
+      float vfac = 1.f;
+      if (b == 0) {
+        if (!sm100::mbar_wait(&info_full[j % kInfo], (uint32_t)((j / kInfo) & 1), abort_flag, a.err)) { ok = false; break; }
+        const Info* I = &info[j % kInfo];
+        // positive even for a zero scale (or one that underflows): masked scores are -inf, and
+        // -inf * 0 would be NaN
+        sc = rowsc * I->kref;
+        if (sc < 1.17549435e-38f) sc = 1.17549435e-38f;
+        vfac = I->vfac;
+        holes = I->holes;
+        vref = I->vref;
+      }
+      const uint32_t s_tmem = s_col + 64u * b;
+      if (!sm100::mbar_wait(&s_full[2 * t + b], (uint32_t)(j & 1), abort_flag, a.err)) { ok = false; break; }
       sm100::tc_fence_after();
-      uint32_t sr[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) sm100::tmem_ld_32x32b_x32(s_tmem + c * 32, sr[c]);
+      uint32_t sr[2][32];
+      sm100::tmem_ld_32x32b_x32(s_tmem, sr[0]);
+      sm100::tmem_ld_32x32b_x32(s_tmem + 32, sr[1]);
       sm100::tmem_ld_wait();
-      if (__builtin_expect(k0 + BLK - 1 > kmax || holes != 0, 0)) {
+      // Rare paths are marked so: code laid out in line with the common one costs instruction
+      // fetches on every block.
+      if (__builtin_expect(k0 + kHalf - 1 > kmax || holes != 0, 0)) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           const int left = kmax + 1 - (k0 + c * 32);  // keys of the chunk that the row sees
           uint32_t seen = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
-          if ((holes >> (2 * c)) & 1) seen &= 0xFFFF0000u;
-          if ((holes >> (2 * c)) & 2) seen &= 0x0000FFFFu;
+          const uint32_t hole = holes >> (4 * b + 2 * c);
+          if (hole & 1) seen &= 0xFFFF0000u;
+          if (hole & 2) seen &= 0x0000FFFFu;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((seen >> i) & 1)) sr[c][i] = __float_as_uint(-INFINITY);
+          for (int e = 0; e < 32; ++e)
+            if (!((seen >> e) & 1)) sr[c][e] = __float_as_uint(-INFINITY);
         }
       }
-      // row max: eight independent chains of three-input maxima
-      float mx8[8];
+      // row max: four independent chains of three-input maxima
+      float mx4[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 4; ++k) {
         const uint32_t* v = &sr[k >> 1][(k & 1) * 16];
         float m = max3f(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
 #pragma unroll
-        for (int i = 3; i + 1 < 16; i += 2) m = max3f(m, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-        mx8[k] = fmaxf(m, __uint_as_float(v[15]));
+        for (int e = 3; e + 1 < 16; e += 2) m = max3f(m, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+        mx4[k] = fmaxf(m, __uint_as_float(v[15]));
       }
-      const float mx = max3f(max3f(mx8[0], mx8[1], mx8[2]), max3f(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
-      const float m_blk = mx * sc;
+      const float m_blk = fmaxf(max3f(mx4[0], mx4[1], mx4[2]), mx4[3]) * sc;
       const bool grow = m_blk > m_used + kRescaleThreshold;
       const float m_prev = m_used;
       if (grow) m_used = m_blk;
       const float m_ref = m_used == -INFINITY ? 0.f : m_used;
       const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(-m_ref, -m_ref);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), sc2, nm2);
+        for (int e = 0; e < 16; ++e) {
+          float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])), sc2, nm2);
           x.x = sm100::ex2_approx(x.x);
           x.y = sm100::ex2_approx(x.y);
-          sr[c][2 * i] = __float_as_uint(x.x);
-          sr[c][2 * i + 1] = __float_as_uint(x.y);
-          pk[i] = pack_f16(x.x, x.y);
+          sr[c][2 * e] = __float_as_uint(x.x);
+          sr[c][2 * e + 1] = __float_as_uint(x.y);
+          pk[e] = pack_f16(x.x, x.y);
         }
         sm100::tmem_st_32x32b_x16(s_tmem + c * 16, pk);
       }
       float alpha = 1.f;
-      if (__builtin_expect(__any_sync(0xffffffffu, (grow || vfac != 1.f) && j > 0), 0)) {
+      if (__builtin_expect(__any_sync(0xffffffffu, (grow || vfac != 1.f) && i > 0), 0)) {
         alpha = grow ? exp2f(m_prev - m_blk) : 1.f;
-        // PV_t(j-1) (and, by commit order, every earlier PV of this tile) must be complete.
-        if (!sm100::mbar_wait(&pv_done[t], (uint32_t)((j - 1) & 1), abort_flag, a.err)) { ok = false; break; }
+        // PV_t(i-1) must be complete (PV_t(i-2) is: S_t(i) was issued after it).
+        if (!sm100::mbar_wait(&pv_done[t], (uint32_t)((i - 1) & 1), abort_flag, a.err)) { ok = false; break; }
         sm100::tc_fence_after();
         const float f = alpha * vfac;
 #pragma unroll 1
@@ -609,24 +622,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           sm100::tmem_ld_32x32b_x32(o_tmem + c * 32, x);
           sm100::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
           sm100::tmem_st_32x32b_x32(o_tmem + c * 32, x);
         }
       }
       sm100::tmem_st_wait();
       sm100::tc_fence_before();
-      sm100::mbar_arrive(&p_full[t]);
+      sm100::mbar_arrive(&p_full[2 * t + b]);
+      // the row sum is taken after P is published, off the path to the next product
       float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          sum[i & 3] =
-              __fadd2_rn(sum[i & 3], make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])));
+        for (int e = 0; e < 16; ++e)
+          sum[e & 3] =
+              __fadd2_rn(sum[e & 3], make_float2(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])));
       const float2 s2 = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
       l = l * alpha + (s2.x + s2.y);
     }
-    if (ok && mine > 0) ok = sm100::mbar_wait(&pv_done[t], (uint32_t)((mine - 1) & 1), abort_flag, a.err);
+    // The last product, by a barrier of its own: pv_done may be one or two phases on by now, and a
+    // wait tells neighbouring phases apart by parity alone.
+    if (ok && mine > 0) ok = sm100::mbar_wait(&done_bar[t], 0, abort_flag, a.err);
     sm100::tc_fence_after();
     if (ok) {
       const bool whole = sa.splits == 1;
@@ -748,13 +764,6 @@ __global__ void __launch_bounds__(128) kv_split_combine(AttnArgs a, int splits) 
 template <typename T, int CODE, int D>
 int go(const AttnArgs& a, int splits, cudaStream_t st) {
   auto k = prompt_kernel<T, CODE, D>;
-  static std::atomic<int> regs_ok{0};
-  if (regs_ok.load() == 0) {
-    cudaFuncAttributes fa;
-    NTB_CUDA(cudaFuncGetAttributes(&fa, k));
-    regs_ok.store(fa.numRegs >= kLaunchRegs ? 1 : -1);
-  }
-  NTB_UNSUP(regs_ok.load() == 1, "attention kernel built with fewer than %d registers per thread", kLaunchRegs);
   NTB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL));
   SplitArgs sa;
   sa.splits = splits;

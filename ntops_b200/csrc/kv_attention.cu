@@ -320,8 +320,8 @@ int fill(const NtbTensor* q, const NtbKvCache* cache, const NtbTensor* table, At
 }
 
 // The kernel that takes a call.  Up to 32 packed rows the decode kernel goes over the keys once for
-// each 16: 41 us against the prompt kernel's 51 for 32 rows over 32768 keys (8 kv heads of 128), 71
-// against 83 for 16 batch rows of 4096; with 48 rows it is 53 against 51 and 100 against 84.
+// each 16: 37 us against the prompt kernel's 51 for 32 rows over 32768 keys (8 kv heads of 128), 63
+// against 80 for 16 batch rows of 4096; a third pass for 48 rows makes it the slower one.
 enum class Path { generic, decode, prompt };
 Path path_of(const AttnArgs& a, int dtype) {
   if (!tensor_cores_take(a, dtype)) return Path::generic;

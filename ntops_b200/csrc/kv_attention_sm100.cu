@@ -21,7 +21,7 @@
 //
 // What bounds it: the exponentials (2 x 128 x 128 of them a block on a 16-per-clock unit: 2048
 // cycles, the products' time as well).  Where one wave of blocks would leave SMs idle, several
-// blocks share a tile's keys and kv_split_combine joins them.
+// blocks share a tile's keys, cut evenly by the lengths, and kv_split_combine joins them.
 #include <algorithm>
 #include <type_traits>
 
@@ -141,26 +141,90 @@ __device__ __forceinline__ int row_of(int i) {
 }
 
 struct SplitArgs {
-  int splits;   // blocks that share a segment's keys
+  int blocks;   // 0: a block for each segment; else segments are cut into about so many pieces
   int box;      // tokens of a TMA box
   int t_shift;  // log2 of the page size, or -1
   int q_vec, o_vec;
 };
 
-// The segment of a block: heavy (late) row tiles of all batch rows and heads first.
+// A piece of a segment: part `split` of `splits` of its keys.
 struct Where {
-  int b, head, tile, split;
+  int b, head, tile, split, splits;
 };
-__device__ __forceinline__ Where where_is(const AttnArgs& a, int splits, int64_t idx) {
+
+// Without cutting: heavy (late) row tiles of all batch rows and heads first.
+__device__ __forceinline__ Where where_is(const AttnArgs& a, int64_t idx) {
   Where w;
-  w.split = (int)(idx % splits);
-  idx /= splits;
+  w.split = 0;
+  w.splits = 1;
   w.head = (int)(idx % a.c.H);
   idx /= a.c.H;
   w.b = a.b0 + (int)(idx % a.nb);
   w.tile = a.tiles - 1 - (int)(idx / a.nb);
   return w;
 }
+
+// With cutting, which the host chooses where there are fewer segments than SMs (so fewer batch rows
+// too): pieces of at most `target` key blocks, the smallest that gives no more than `blocks`
+// pieces, so that one wave of them is as even as the lengths allow.  One warp derives it from the
+// lengths.  Batch row b has pieces [first(b), first(b + 1)), its segments' splits fastest.
+constexpr int kCutRows = 5;  // batch rows a lane holds: 160 rows at most
+struct Cut {
+  int units[kCutRows], target;
+  __device__ __forceinline__ Cut(const AttnArgs& a, int blocks) {
+    const int lane = threadIdx.x & 31, segs = a.tiles * a.c.H;
+    int total = 0;
+#pragma unroll
+    for (int k = 0; k < kCutRows; ++k) {
+      const int b = lane + 32 * k;
+      units[k] = b < a.nb ? row_units(a, a.b0 + b) : 0;
+      total += units[k];
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    target = max(4, (int)quotient((int64_t)total * segs + blocks - 1, blocks));
+    for (int tries = 0; tries < 32 && pieces(a.nb) * segs > blocks; ++tries) target += (target + 7) / 8;
+  }
+  __device__ __forceinline__ int splits(int k) const { return (units[k] + target - 1) / target; }
+  // pieces of one segment row of the first n batch rows
+  __device__ __forceinline__ int pieces(int n) const {
+    const int lane = threadIdx.x & 31;
+    int s = 0;
+#pragma unroll
+    for (int k = 0; k < kCutRows; ++k)
+      if (lane + 32 * k < n) s += splits(k);
+    return __reduce_add_sync(0xffffffffu, s);
+  }
+  __device__ __forceinline__ int splits_of(int b) const {  // the same for every lane
+    int s = 0;
+#pragma unroll
+    for (int k = 0; k < kCutRows; ++k) {
+      const int v = __shfl_sync(0xffffffffu, splits(k), b & 31);
+      if (k == b >> 5) s = v;
+    }
+    return s;
+  }
+  // b < 0: there is no such piece
+  __device__ __forceinline__ Where at(const AttnArgs& a, int idx) const {
+    const int segs = a.tiles * a.c.H;
+    Where w;
+    w.b = -1;
+    int before = 0;
+    for (int b = 0; b < a.nb; ++b) {
+      const int s = splits_of(b), n = s * segs;
+      if (idx < before + n) {
+        const int r = idx - before;
+        w.b = a.b0 + b;
+        w.splits = s;
+        w.split = r % s;
+        w.head = r / s % a.c.H;
+        w.tile = r / s / a.c.H;
+        return w;
+      }
+      before += n;
+    }
+    return w;
+  }
+};
 
 template <typename T, int CODE, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -192,7 +256,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   Info* info = reinterpret_cast<Info*>(sm + S::INFO);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Where w = where_is(a, sa.splits, blockIdx.x);
+  Where w;
+  if (sa.blocks == 0) {
+    w = where_is(a, blockIdx.x);
+  } else {
+    __shared__ Where mine;
+    if (warp == 0) {
+      const Cut cut(a, sa.blocks);
+      const Where x = cut.at(a, blockIdx.x);
+      if (lane == 0) mine = x;
+    }
+    __syncthreads();
+    w = mine;
+    if (w.b < 0) return;
+  }
   const int len = row_length(a, w.b), start = row_start(a, w.b, len);
   const int r0 = w.tile * kTiles * BLK;
   // Key blocks [jb, jb + n) of this block; tile t takes the first n_t of them.
@@ -208,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       all = max(all, n_t[t]);
     }
   }
-  const int jb = (int)((int64_t)all * w.split / sa.splits), je = (int)((int64_t)all * (w.split + 1) / sa.splits);
+  const int jb = (int)((int64_t)all * w.split / w.splits), je = (int)((int64_t)all * (w.split + 1) / w.splits);
   int n = 0;
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
@@ -558,6 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         vref = I->vref;
       }
       const uint32_t s_tmem = s_col + 64u * b;
+      const bool edge = __any_sync(0xffffffffu, k0 + kHalf - 1 > kmax) || holes != 0;
       if (!sm100::mbar_wait(&s_full[2 * t + b], (uint32_t)(j & 1), abort_flag, a.err)) { ok = false; break; }
       sm100::tc_fence_after();
       uint32_t sr[2][32];
@@ -566,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::tmem_ld_wait();
       // Rare paths are marked so: code laid out in line with the common one costs instruction
       // fetches on every block.
-      if (__builtin_expect(k0 + kHalf - 1 > kmax || holes != 0, 0)) {
+      if (__builtin_expect(edge, 0)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int left = kmax + 1 - (k0 + c * 32);  // keys of the chunk that the row sees
@@ -645,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && mine > 0) ok = sm100::mbar_wait(&done_bar[t], 0, abort_flag, a.err);
     sm100::tc_fence_after();
     if (ok) {
-      const bool whole = sa.splits == 1;
+      const bool whole = w.splits == 1;
       const float f = !whole ? vref : l == 0.f ? 0.f : vref / l;
       const bool none = l == 0.f;  // nothing seen (NaN is not 0)
       float* part = nullptr;
@@ -704,23 +782,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the splits of every row, one warp a row, as combine_kernel does.
+// Joins the pieces of every cut segment's rows, one warp a row, as combine_kernel does.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv_split_combine(AttnArgs a, int splits) {
+__global__ void __launch_bounds__(128) kv_split_combine(AttnArgs a, int blocks) {
   constexpr int E = D / 32;  // channels of a lane
   using V = ew::Vec<float, E>;
   const int lane = threadIdx.x & 31;
-  const int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);  // (segment, row), segments as where_is orders them
-  const int rows = kTiles * BLK;
-  const int64_t seg = job / rows;
-  const int rt = (int)(job % rows);
-  if (seg >= (int64_t)a.nb * a.tiles * a.c.H) return;
-  const Where w = where_is(a, 1, seg);
-  const int r = w.tile * rows + rt;
+  const int rows = kTiles * BLK, segs = a.tiles * a.c.H;
+  const int job = (int)blockIdx.x * 4 + (threadIdx.x >> 5);  // (batch row, tile, head, row of the tile)
+  const int rt = job % rows, seg = job / rows % segs, b = job / rows / segs;
+  if (b >= a.nb) return;
+  const int tile = seg / a.c.H, head = seg % a.c.H, r = tile * rows + rt;
   if (r >= a.rows) return;
+  const Cut cut(a, blocks);  // (lengths are the call's inputs, not the previous kernel's output)
+  const int splits = cut.splits_of(b), first = cut.pieces(b) * segs + seg * splits;
+  if (splits == 1) return;  // its block wrote the output
   grid_dependency_wait();
   const int64_t slot = slot_floats(rows, D);
-  const float* base = a.part + seg * splits * slot;
+  const float* base = a.part + (int64_t)first * slot;
   const int64_t stat = (int64_t)rows * D + 2 * rt;
   float M = -INFINITY;
   for (int c = lane; c < splits; c += 32) M = fmaxf(M, base[c * slot + stat]);
@@ -754,19 +833,22 @@ __global__ void __launch_bounds__(128) kv_split_combine(AttnArgs a, int splits) 
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  T* o = reinterpret_cast<T*>(a.o) + (int64_t)w.b * a.o_b + (int64_t)(w.head * a.group + r % a.group) * a.o_h +
+  T* o = reinterpret_cast<T*>(a.o) + (int64_t)(a.b0 + b) * a.o_b + (int64_t)(head * a.group + r % a.group) * a.o_h +
          (int64_t)(r / a.group) * a.o_s + lane * E;
   const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = cvt<T>(L == 0.f ? 0.f : acc[e] * inv);
 }
 
+// Pieces that segments cut for `blocks` can number: one for each segment more.
+inline int64_t pieces_bound(int64_t segs, int blocks) { return segs + blocks; }
+
 template <typename T, int CODE, int D>
-int go(const AttnArgs& a, int splits, cudaStream_t st) {
+int go(const AttnArgs& a, int blocks, cudaStream_t st) {
   auto k = prompt_kernel<T, CODE, D>;
   NTB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL));
   SplitArgs sa;
-  sa.splits = splits;
+  sa.blocks = blocks;
   sa.box = 16;
   while (sa.box < kHalf && a.c.T % (2 * sa.box) == 0) sa.box *= 2;
   sa.t_shift = -1;
@@ -780,22 +862,22 @@ int go(const AttnArgs& a, int splits, cudaStream_t st) {
   int rc;
   if ((rc = code_map(&tk, a.c.key, a.c, a.c.k_t, a.c.k_h, a.c.k_p, sa.box)) != NTB_OK) return rc;
   if ((rc = code_map(&tv, a.c.value, a.c, a.c.v_t, a.c.v_h, a.c.v_p, sa.box)) != NTB_OK) return rc;
-  const int64_t segs = (int64_t)a.nb * a.tiles * a.c.H, grid = segs * splits;
-  NTB_UNSUP(grid <= 0x7fffffffLL && segs * 64 <= 0x7fffffffLL, "kv_attention: too many query rows");
+  const int64_t segs = (int64_t)a.nb * a.tiles * a.c.H, grid = blocks > 0 ? pieces_bound(segs, blocks) : segs;
+  NTB_UNSUP(grid <= 0x7fffffffLL, "kv_attention: too many query rows");
   k<<<(unsigned)grid, kThreads, Smem<D>::TOTAL, st>>>(tk, tv, a, sa);
   NTB_LAUNCH_CHECK();
-  if (splits > 1)
+  if (blocks > 0)
     NTB_CUDA(launch_dependent(kv_split_combine<T, D>, dim3((unsigned)(segs * kTiles * BLK / 4)), dim3(128), 0, st, a,
-                              splits));
+                              blocks));
   return NTB_OK;
 }
 
-// Blocks that share a segment's keys: as many as one wave of one block an SM holds, each with at
-// least four key blocks of a full table.
-int splits_of(const AttnArgs& a) {
+// Whether segments are cut (into about one piece an SM): only where they are fewer than the SMs, and
+// a full table has more key blocks than the smallest piece.  (The segments of the last launch of a
+// large batch are few too, but sizes are planned for the first, which has most.)
+int cut_blocks(const AttnArgs& a) {
   const int64_t segs = (int64_t)std::min(a.table.B, kMaxBatch) * a.tiles * a.c.H;
-  const int64_t cap = ((int64_t)a.table.M * a.c.T + 4 * BLK - 1) / (4 * BLK);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / segs, cap));
+  return segs < sm_count() && segs <= 32 * kCutRows && (int64_t)a.table.M * a.c.T > 4 * BLK ? sm_count() : 0;
 }
 
 }  // namespace
@@ -804,17 +886,18 @@ void prompt_plan(AttnArgs* a) {
   a->tile = kTiles * BLK;
   a->tiles = (a->rows + a->tile - 1) / a->tile;
   a->unit = BLK;
-  const int splits = splits_of(*a);
+  const int blocks = cut_blocks(*a);
   // combine_kernel is not used: G only sizes the workspace (two slots for each unit of G)
-  a->G = splits > 1 ? (int)(((int64_t)std::min(a->table.B, kMaxBatch) * a->tiles * a->c.H * splits + 1) / 2) : 0;
+  const int64_t segs = (int64_t)std::min(a->table.B, kMaxBatch) * a->tiles * a->c.H;
+  a->G = blocks > 0 ? (int)((pieces_bound(segs, blocks) + 1) / 2) : 0;
 }
 
 int prompt_launch(const AttnArgs& a, int dtype, cudaStream_t st) {
-  const int splits = splits_of(a);
+  const int blocks = cut_blocks(a);
   auto by_d = [&](auto t, auto code) -> int {
     using T = decltype(t);
     constexpr int CODE = decltype(code)::value;
-    return a.c.D == 128 ? go<T, CODE, 128>(a, splits, st) : go<T, CODE, 64>(a, splits, st);
+    return a.c.D == 128 ? go<T, CODE, 128>(a, blocks, st) : go<T, CODE, 64>(a, blocks, st);
   };
   using E = std::integral_constant<int, NTB_F8E4M3>;
   using I = std::integral_constant<int, NTB_I8>;

@@ -170,20 +170,21 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(AttnArgs a)
   const int64_t job = (int64_t)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
   const int rt = (int)(job % a.tile);
   const int64_t sg = job / a.tile;
-  const int x = (int)(sg / line.segs), seg = (int)(sg % line.segs);
-  if (x >= a.nb) return;
+  const int x = (int)min(sg / line.segs, (int64_t)a.nb - 1), seg = (int)(sg % line.segs);
   const int tile = seg / a.c.H, head = seg % a.c.H, r = tile * a.tile + rt;
-  if (r >= a.rows) return;
   const int units = pre[x + 1] - pre[x];
   const int64_t u0 = (int64_t)pre[x] * line.segs + (int64_t)seg * units;
   const int c0 = line.owner(u0), c1 = line.owner(u0 + units - 1);
-  if (c0 == c1) return;  // whole: its block wrote the output
   const int D = a.c.D, b = a.b0 + x;
   const int64_t slot = slot_floats(a.tile, D);
   const int first = 2 * c0 + (line.begin(c0) < u0 ? 1 : 0);
   auto piece = [&](int c) { return a.part + (int64_t)(c == c0 ? first : 2 * c) * slot; };
   const int64_t stat = (int64_t)a.tile * D + 2 * rt;  // of the row's max and sum in a slot
+  // Before any return: a grid that ended early would let the stream's next kernel overtake the
+  // previous one.
   grid_dependency_wait();
+  // (one piece: whole, its block wrote the output)
+  if (sg >= (int64_t)a.nb * line.segs || r >= a.rows || c0 == c1) return;
   float M = -INFINITY;
   for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, piece(c)[stat]);
 #pragma unroll

@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
     *abort_flag = 0;
     sm100::fence_mbar_init();
   }
+  grid_dependency_wait();
   grid_dependency_launch();  // the joining kernel may start; it waits for this one before it reads
   prefix_units<kThreads>(a, pre);  // (its barriers publish the mbarriers)
   const Line line(a, pre);
@@ -590,8 +591,7 @@ int go(const AttnArgs& a, cudaStream_t st, int* blocks) {
   int rc;
   if ((rc = code_map(&tk, a.c.key, a.c, a.c.k_t, a.c.k_h, a.c.k_p, box)) != NTB_OK) return rc;
   if ((rc = code_map(&tv, a.c.value, a.c, a.c.v_t, a.c.v_h, a.c.v_p, box)) != NTB_OK) return rc;
-  k<<<a.G, kThreads, smem, st>>>(tk, tv, a, pow2_page ? shift : -1, box, q_vec, o_vec);
-  NTB_LAUNCH_CHECK();
+  NTB_CUDA(launch_dependent(k, dim3(a.G), dim3(kThreads), smem, st, tk, tv, a, pow2_page ? shift : -1, box, q_vec, o_vec));
   return NTB_OK;
 }
 

@@ -791,13 +791,13 @@ __global__ void __launch_bounds__(128) kv_split_combine(AttnArgs a, int blocks) 
   const int rows = kTiles * BLK, segs = a.tiles * a.c.H;
   const int job = (int)blockIdx.x * 4 + (threadIdx.x >> 5);  // (batch row, tile, head, row of the tile)
   const int rt = job % rows, seg = job / rows % segs, b = job / rows / segs;
+  const Cut cut(a, blocks);  // (lengths are the call's inputs, not the previous kernel's output)
+  grid_dependency_wait();    // before any return: see combine_kernel
   if (b >= a.nb) return;
   const int tile = seg / a.c.H, head = seg % a.c.H, r = tile * rows + rt;
   if (r >= a.rows) return;
-  const Cut cut(a, blocks);  // (lengths are the call's inputs, not the previous kernel's output)
   const int splits = cut.splits_of(b), first = cut.pieces(b) * segs + seg * splits;
   if (splits == 1) return;  // its block wrote the output
-  grid_dependency_wait();
   const int64_t slot = slot_floats(rows, D);
   const float* base = a.part + (int64_t)first * slot;
   const int64_t stat = (int64_t)rows * D + 2 * rt;

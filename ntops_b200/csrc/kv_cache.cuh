@@ -96,7 +96,9 @@ __device__ __forceinline__ float decode1(uint8_t c) {
 
 // ------------------------------------------------------------- programmatic launch --------
 // A kernel launched with programmatic stream serialisation may start before its predecessor
-// ends; this waits until the predecessor has finished and its writes are visible.
+// ends; this waits until the predecessor has finished and its writes are visible.  Every block of
+// such a kernel calls it, before it returns or touches memory that the stream's earlier work
+// touches.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

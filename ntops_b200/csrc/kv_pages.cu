@@ -11,6 +11,7 @@
 
 #include "kv_cache.cuh"
 #include "rowstage.cuh"
+#include "sm100.cuh"
 
 namespace ntb {
 namespace kv {
@@ -89,6 +90,101 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(CopyArgs a) {
   }
 }
 
+// Dense pages move through shared memory by bulk copies alone: one thread keeps kBulkStages chunks
+// going, loads on one side and stores on the other, and no register or issue slot sees a byte.
+// The block's second warp copies the scales.
+constexpr int kBulkStages = 3;
+constexpr int kBulkChunk = 32 * 1024;
+
+__global__ void __launch_bounds__(64) copy_bulk_kernel(CopyArgs a, unsigned int* err) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kBulkStages];
+  __shared__ int abort_flag;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kBulkStages; ++s) sm100::mbar_init(&full[s], 1);
+    abort_flag = 0;
+    sm100::fence_mbar_init();
+  }
+  __syncthreads();
+  grid_dependency_wait();
+  const int pairs = a.count == nullptr ? a.pairs : min(max(*a.count, 0), a.pairs);
+  auto pages = [&](int k, int* from, int* to) {
+    *from = a.src[k * a.src_s];
+    *to = a.dst[k * a.dst_s];
+    return (unsigned)*from < (unsigned)a.P && (unsigned)*to < (unsigned)a.P && *from != *to;
+  };
+  if (threadIdx.x >= 32) {
+    const int per_pair = a.L * 2 * a.H, n = pairs * per_pair;
+    for (int i = blockIdx.x * 32 + (threadIdx.x & 31); i < n; i += gridDim.x * 32) {
+      const int k = i / per_pair, r = i - k * per_pair, h = r % a.H, w = (r / a.H) & 1, l = r / a.H >> 1;
+      int from, to;
+      if (!pages(k, &from, &to)) continue;
+      float* sc = a.scale[w] + (int64_t)l * a.s_l[w] + (int64_t)h * a.s_h[w];
+      sc[(int64_t)to * a.s_p[w]] = sc[(int64_t)from * a.s_p[w]];
+    }
+    return;
+  }
+  if (threadIdx.x != 0) return;
+  const int chunks = (int)((a.block + kBulkChunk - 1) / kBulkChunk), per_pair = a.L * 2 * chunks;
+  const int items = pairs * per_pair;
+  // The chunk of item `it`: where it goes and its bytes (0: a pair out of range).
+  auto chunk = [&](int it, const uint8_t** s, uint8_t** d) -> uint32_t {
+    const int k = it / per_pair, r = it - k * per_pair, c = r % chunks, w = (r / chunks) & 1, l = r / chunks >> 1;
+    int from, to;
+    if (!pages(k, &from, &to)) return 0;
+    const int64_t at = (int64_t)l * a.c_l[w] + (int64_t)c * kBulkChunk;
+    *s = a.code[w] + at + (int64_t)from * a.c_p[w];
+    *d = a.code[w] + at + (int64_t)to * a.c_p[w];
+    return (uint32_t)min((int64_t)kBulkChunk, a.block - (int64_t)c * kBulkChunk);
+  };
+  const int mine = (int)blockIdx.x < items ? (items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  uint8_t* to[kBulkStages];
+  uint32_t bytes[kBulkStages];
+  auto load = [&](int i, int st) {
+    const uint8_t* from = nullptr;
+    const uint32_t n = chunk(blockIdx.x + i * (int)gridDim.x, &from, &to[st]);
+    bytes[st] = n;
+    sm100::mbar_arrive_expect_tx(&full[st], n);
+    if (n > 0)
+      asm volatile(
+          "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+              sm100::smem_u32(ring + st * kBulkChunk)),
+          "l"(from), "r"(n), "r"(sm100::smem_u32(&full[st]))
+          : "memory");
+  };
+  int loaded = 0;
+#pragma unroll
+  for (int i = 0; i < kBulkStages - 1; ++i)
+    if (i < mine) {
+      load(i, i);
+      ++loaded;
+    }
+  bool ok = true;
+  for (int i0 = 0; ok && i0 < mine; i0 += kBulkStages) {
+#pragma unroll
+    for (int st = 0; st < kBulkStages; ++st) {
+      const int i = i0 + st;
+      if (i >= mine || !ok) break;
+      ok = sm100::mbar_wait(&full[st], (uint32_t)((i / kBulkStages) & 1), &abort_flag, err);
+      if (!ok) break;
+      if (bytes[st] > 0)
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to[st]),
+                     "r"(sm100::smem_u32(ring + st * kBulkChunk)), "r"(bytes[st])
+                     : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      if (i + kBulkStages - 1 < mine) {  // into the slot of the previous item, once its store has read it
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        load(i + kBulkStages - 1, (st + kBulkStages - 1) % kBulkStages);
+        ++loaded;
+      }
+    }
+  }
+  if (!ok)  // a wait gave up: the loads under way land before the shared memory goes
+    for (int i = max(loaded - kBulkStages, 0); i < loaded; ++i)
+      sm100::mbar_wait_unwind(&full[i % kBulkStages], (uint32_t)((i / kBulkStages) & 1));
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
 int fill_copy(const NtbKvCache* c, CopyArgs* a) {
   Layer l;
   int rc = check_cache(c, true, &l);
@@ -121,6 +217,14 @@ int launch_copy(const CopyArgs& a, cudaStream_t st) {
   const int64_t most = (int64_t)a.pairs * a.L * 2 * chunks;
   if (most == 0) return NTB_OK;
   NTB_UNSUP(most <= 0x3fffffffLL, "too many bytes to copy in one call");
+  if (a.dense) {
+    constexpr int kSmem = kBulkStages * kBulkChunk;
+    NTB_CUDA(cudaFuncSetAttribute(copy_bulk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    const int64_t items = (int64_t)a.pairs * a.L * 2 * ((a.block + kBulkChunk - 1) / kBulkChunk);
+    const int64_t grid = std::min<int64_t>(items, resident_blocks((const void*)copy_bulk_kernel, 64, kSmem));
+    NTB_CUDA(launch_dependent(copy_bulk_kernel, dim3((unsigned)grid), dim3(64), kSmem, st, a, device_error_ptr()));
+    return NTB_OK;
+  }
   const int64_t grid = std::min<int64_t>(most, resident_blocks((const void*)copy_kernel, kCopyThreads, 0));
   NTB_CUDA(launch_dependent(copy_kernel, dim3((unsigned)grid), dim3(kCopyThreads), 0, st, a));
   return NTB_OK;

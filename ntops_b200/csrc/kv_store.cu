@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(GT == 32 ? 128 : GT, GT == 256 ? 4 : 8) store_
   constexpr int kThreads = GT == 32 ? 128 : GT;
   using V = ew::Vec<T, VE>;
   __shared__ float red[kThreads / 32];
+  grid_dependency_wait();
   const int64_t unit = (int64_t)blockIdx.x * (kThreads / GT) + (GT == 32 ? threadIdx.x / 32 : 0);
   if (unit >= a.units) return;  // whole warps (GT 32) or no block (GT = block) leave here
   const int lane = GT == 32 ? threadIdx.x % 32 : threadIdx.x;
@@ -198,10 +199,11 @@ int launch_store(const StoreArgs& a, cudaStream_t st) {
   const bool warp = vecs <= 32 * kHeld;
   const int64_t grid = warp ? (a.units + 3) / 4 : a.units;
   NTB_UNSUP(grid <= 0x7fffffffLL, "kv_store: too many pages in one call");
-  if (warp) store_kernel<T, CODE, 32, VEC><<<(unsigned)grid, 128, 0, st>>>(a);
-  else if (vecs <= 128 * kHeld) store_kernel<T, CODE, 128, VEC><<<(unsigned)grid, 128, 0, st>>>(a);
-  else store_kernel<T, CODE, 256, VEC><<<(unsigned)grid, 256, 0, st>>>(a);
-  NTB_LAUNCH_CHECK();
+  cudaError_t rc;
+  if (warp) rc = launch_dependent(store_kernel<T, CODE, 32, VEC>, dim3((unsigned)grid), dim3(128), 0, st, a);
+  else if (vecs <= 128 * kHeld) rc = launch_dependent(store_kernel<T, CODE, 128, VEC>, dim3((unsigned)grid), dim3(128), 0, st, a);
+  else rc = launch_dependent(store_kernel<T, CODE, 256, VEC>, dim3((unsigned)grid), dim3(256), 0, st, a);
+  NTB_CUDA(rc);
   return NTB_OK;
 }
 

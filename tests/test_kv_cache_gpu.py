@@ -89,6 +89,13 @@ ATTEND = [
     ([300, 70], 70, 4, 1, 64, 64, I8, F16),
     ([260], 130, 8, 8, 128, 32, E4M3, F16),
     ([129, 640], 65, 16, 2, 128, 128, I8, BF16),
+    ([500, 49], 1, 8, 2, 128, 48, E4M3, BF16),  # pages of 16-token groups that are no power of two
+    ([500, 49], 24, 4, 2, 64, 48, I8, F16),
+    ([385, 97], 40, 8, 2, 128, 48, E4M3, BF16),
+    ([700, 257], 1, 4, 2, 64, 256, I8, BF16),
+    ([700, 257], 45, 4, 2, 128, 256, E4M3, F16),
+    ([333, 20], 8, 8, 2, 128, 16, I8, BF16),    # 32 rows: the most of the few-row kernel
+    ([333, 20], 33, 2, 2, 128, 16, I8, BF16),   # one more
 ]
 
 
@@ -253,6 +260,22 @@ def test_attention_long_uneven_rows(sq):
     got = kc.attention(q.to(DEV), cache.layer(0), table.to(DEV), n.to(DEV))
     _check_attention(got, q, cache, 0, table, n, 1 / math.sqrt(d), True)
     assert torch.equal(got, kc.attention(q.to(DEV), cache.layer(0), table.to(DEV), n.to(DEV)))
+
+
+def test_no_wait_gave_up():
+    """The kernels' bounded waits (the copy ring, the tensor-core pipeline) end in time: a device error
+    word would say otherwise."""
+    from ntops_b200 import _lib
+
+    cache = _random_cache(1, 130, 2, 64, 128, E4M3)
+    table = _table([4000, 4100], 64, 130)
+    n = torch.tensor([4000, 4100], dtype=torch.int32, device=DEV)
+    for sq in (1, 8, 40, 300):
+        q = torch.randn(2, 8, sq, 128, device=DEV).to(BF16)
+        first = kc.attention(q, cache.layer(0), table.to(DEV), n)
+        for _ in range(20):
+            assert torch.equal(kc.attention(q, cache.layer(0), table.to(DEV), n), first)
+    assert _lib.load().ntb_check_device_error(None) == 0
 
 
 def test_attention_of_nothing():

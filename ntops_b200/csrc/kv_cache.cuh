@@ -70,9 +70,14 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 template <int CODE>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
   if constexpr (CODE == NTB_F8E4M3) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
+    uint32_t r;  // (the conversion's first source is the upper byte)
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+        "mov.b32 %0, {l, h};\n\t}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
   } else {
     auto q = [](float x) -> uint32_t {
       // a NaN loses both comparisons of fminf / fmaxf, so it is set to 0 first

@@ -8,6 +8,10 @@
 // One group of threads owns a (b, h, page) of the keys or of the values, so nothing is shared
 // between groups: no atomics, one launch.  The page's new elements are loaded once, as 16-byte
 // vectors kept in registers between the maximum and the rounding.
+//
+// What bounds it: HBM for prompts (eight of 4096 tokens, 8 heads of 128, bf16: 37.5 us, 0.82 of the
+// copy rate; instruction issue is 69 % busy beside it), the launch for single tokens (64 rows:
+// 3.0 us back to back).
 #include <algorithm>
 #include <type_traits>
 
@@ -25,7 +29,7 @@ struct StoreArgs {
   const int *start, *counts;                       // counts may be null: S for every row
   int64_t st_s, ct_s;
   int B, S, cover;                                 // cover: pages that S tokens can touch
-  int64_t units;                                   // 2 * B * H * cover
+  int units;                                       // 2 * B * H * cover
 };
 
 constexpr int kHeld = 8;  // 16-byte vectors a thread keeps in registers
@@ -54,7 +58,8 @@ __device__ __forceinline__ float finite_abs(float x) {
 }
 
 // The vectors lane, lane + GT, ... of a page's rows: row and vector within the row, stepped
-// without a division.
+// without a division.  (A form for groups that cover whole rows, with no step within the row, has a
+// tenth fewer instructions and measured slower: 42 us against 37.5 on eight 4096-token prompts.)
 struct Walk {
   int r, v, i;
   __device__ __forceinline__ Walk(int lane, int vpr) : r(lane / vpr), v(lane - r * vpr), i(lane) {}
@@ -77,15 +82,12 @@ __global__ void __launch_bounds__(GT == 32 ? 128 : GT, GT == 256 ? 4 : 8) store_
   using V = ew::Vec<T, VE>;
   __shared__ float red[kThreads / 32];
   grid_dependency_wait();
-  const int64_t unit = (int64_t)blockIdx.x * (kThreads / GT) + (GT == 32 ? threadIdx.x / 32 : 0);
+  const int unit = (int)blockIdx.x * (kThreads / GT) + (GT == 32 ? (int)threadIdx.x / 32 : 0);
   if (unit >= a.units) return;  // whole warps (GT 32) or no block (GT = block) leave here
   const int lane = GT == 32 ? threadIdx.x % 32 : threadIdx.x;
   // heads fastest: neighbouring groups read neighbouring rows of a [B, S, H, D] input
-  int64_t u = unit / a.c.H;
-  const int h = (int)(unit - u * a.c.H);
-  const int which = (int)(u & 1);
-  u >>= 1;
-  const int b = (int)(u / a.cover), j = (int)(u - (int64_t)b * a.cover);
+  const int u = unit / a.c.H, h = unit - u * a.c.H;
+  const int which = u & 1, b = (u >> 1) / a.cover, j = (u >> 1) - b * a.cover;
   const int start = a.start[(int64_t)b * a.st_s];
   const int n = a.counts == nullptr ? a.S : min(max(a.counts[(int64_t)b * a.ct_s], 0), a.S);
   const int T_ = a.c.T, D = a.c.D;
@@ -195,16 +197,17 @@ __global__ void __launch_bounds__(GT == 32 ? 128 : GT, GT == 256 ? 4 : 8) store_
 template <typename T, int CODE, bool VEC>
 int launch_store(const StoreArgs& a, cudaStream_t st) {
   // A warp a page while its registers hold the page's new elements, else a block.
-  const int64_t vecs = (int64_t)std::min(a.S, a.c.T) * (a.c.D / (VEC ? 16 / (int)sizeof(T) : 1));
-  const bool warp = vecs <= 32 * kHeld;
-  const int64_t grid = warp ? (a.units + 3) / 4 : a.units;
-  NTB_UNSUP(grid <= 0x7fffffffLL, "kv_store: too many pages in one call");
-  cudaError_t rc;
-  if (warp) rc = launch_dependent(store_kernel<T, CODE, 32, VEC>, dim3((unsigned)grid), dim3(128), 0, st, a);
-  else if (vecs <= 128 * kHeld) rc = launch_dependent(store_kernel<T, CODE, 128, VEC>, dim3((unsigned)grid), dim3(128), 0, st, a);
-  else rc = launch_dependent(store_kernel<T, CODE, 256, VEC>, dim3((unsigned)grid), dim3(256), 0, st, a);
-  NTB_CUDA(rc);
-  return NTB_OK;
+  const int vpr = a.c.D / (VEC ? 16 / (int)sizeof(T) : 1);
+  const int64_t vecs = (int64_t)std::min(a.S, a.c.T) * vpr;
+  auto go = [&](auto gt) -> int {
+    constexpr int GT = decltype(gt)::value, threads = GT == 32 ? 128 : GT;
+    const int grid = GT == 32 ? (a.units + 3) / 4 : a.units;
+    NTB_CUDA(launch_dependent(store_kernel<T, CODE, GT, VEC>, dim3((unsigned)grid), dim3(threads), 0, st, a));
+    return NTB_OK;
+  };
+  if (vecs <= 32 * kHeld) return go(std::integral_constant<int, 32>{});
+  if (vecs <= 128 * kHeld) return go(std::integral_constant<int, 128>{});
+  return go(std::integral_constant<int, 256>{});
 }
 
 template <typename T>
@@ -306,7 +309,9 @@ extern "C" int ntb_kv_store(const NtbKvCache* cache, const NtbTensor* key, const
   a.counts = counts ? reinterpret_cast<const int*>(counts->data) : nullptr;
   a.ct_s = counts ? counts->stride[0] : 0;
   a.cover = (int)std::min<int64_t>(((int64_t)a.S + a.c.T - 2) / a.c.T + 1, a.table.M);
-  a.units = 2ll * a.B * a.c.H * a.cover;
+  const int64_t units = 2ll * a.B * a.c.H * a.cover;
+  NTB_UNSUP(units <= 0x7fffff00LL, "kv_store: too many pages in one call");
+  a.units = (int)units;
   // vectors: 16-byte input rows; codes written 4 (fp32) or 8 (16-bit) at a time
   const int es = dtype_size(key->dtype), ve = 16 / es;
   auto in_ok = [&](const NtbTensor* t) {

@@ -94,7 +94,7 @@ _PB = ctypes.c_char_p  # a descriptor as packed bytes (pack_desc), read by the c
 _VP = ctypes.c_void_p
 
 # NtbTensor layouts by rank: pointer, dtype, ndim, the sizes, the strides (each padded to MAX_DIMS).
-_PACK = tuple(
+PACK = tuple(
     struct.Struct(f"Pii{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x").pack if n else struct.Struct("Pii128x").pack
     for n in range(MAX_DIMS + 1)
 )
@@ -104,7 +104,7 @@ def pack_desc(t, code):
     """The bytes of t's NtbTensor with the given dtype code: a quarter of the time that filling the
     ctypes structure takes, for calls whose kernels last a few microseconds.  No checks."""
     n = t.dim()
-    return _PACK[n](t.data_ptr(), code, n, *t.shape, *t.stride())
+    return PACK[n](t.data_ptr(), code, n, *t.shape, *t.stride())
 
 _SIGNATURES = {
     "ntb_version": ([], ctypes.c_int),

@@ -273,8 +273,7 @@ int generic_any(const AttnArgs& a, int dtype, cudaStream_t st, int* blocks) {
 }
 
 int combine_launch(const AttnArgs& a, int dtype, cudaStream_t st) {
-  // One unit for every segment at most: nothing can be cut.
-  if ((int64_t)a.table.M * a.c.T <= a.unit) return NTB_OK;
+  if ((int64_t)a.table.M * a.c.T <= a.unit) return NTB_OK;  // nothing can be cut
   const int64_t jobs = (int64_t)a.nb * a.tiles * a.c.H * a.tile, grid = (jobs + kCombineWarps - 1) / kCombineWarps;
   const size_t smem = sizeof(int) * (a.nb + 1);
   NTB_UNSUP(grid <= 0x7fffffffLL, "kv_attention: too many query rows");
@@ -344,7 +343,12 @@ int plan(AttnArgs* a, int dtype) {
   return generic_any(*a, dtype, nullptr, &a->G);
 }
 
-int64_t part_bytes(const AttnArgs& a) { return 2ll * a.G * slot_floats(a.tile, a.c.D) * (int64_t)sizeof(float); }
+// A table of one unit a row cannot be cut.
+bool never_cut(const AttnArgs& a) { return (int64_t)a.table.M * a.c.T <= a.unit; }
+
+int64_t part_bytes(const AttnArgs& a) {
+  return never_cut(a) ? 0 : 2ll * a.G * slot_floats(a.tile, a.c.D) * (int64_t)sizeof(float);
+}
 
 }  // namespace
 

@@ -34,7 +34,7 @@ _QUERY_TYPES = {t: _lib.DTYPE_CODES[t] for t in (torch.bfloat16, torch.float16, 
 _F32 = _lib.DTYPE_CODES[torch.float32]
 _I32 = _lib.DTYPE_CODES[torch.int32]
 _INT = {torch.int32: _I32}
-_pack = _lib.pack_desc
+_pack, _PACK = _lib.pack_desc, _lib.PACK
 
 
 def _tensor(t, name, device, codes, ndim):
@@ -47,9 +47,10 @@ def _tensor(t, name, device, codes, ndim):
     code = codes.get(t.dtype)
     if code is None:
         raise RuntimeError(f"{name} must be one of {', '.join(str(d) for d in codes)}, got {t.dtype}")
-    if t.dim() != ndim:
-        raise RuntimeError(f"{name} must be {ndim}-D, got {t.dim()}-D")
-    return _pack(t, code)
+    shape = t.shape
+    if len(shape) != ndim:
+        raise RuntimeError(f"{name} must be {ndim}-D, got {len(shape)}-D")
+    return _PACK[ndim](t.data_ptr(), code, ndim, *shape, *t.stride())
 
 
 def _call(what, fn, index, *args):
@@ -172,8 +173,6 @@ def attention(query, layer, block_table, lengths, scale=None, is_causal=True, st
     td = _tensor(block_table, "block_table", c.device, _INT, 2)
     ld = _tensor(lengths, "lengths", c.device, _INT, 1)
     sd = None if start is None else _tensor(start, "start", c.device, _INT, 1)
-    if query.shape[-1] > 1 and query.stride(-1) != 1:
-        raise RuntimeError("query must have a unit inner stride")
     if scale is None:
         scale = 1 / math.sqrt(query.shape[-1])
     L = lib()
@@ -185,9 +184,9 @@ def attention(query, layer, block_table, lengths, scale=None, is_causal=True, st
             _lib.check(L.ntb_kv_attention_workspace(qd, c._desc, td, ctypes.byref(n)), "kv_attention")
         nbytes = c._workspace[sizes] = n.value
     output = torch.empty_like(query)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=c.device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=c.device) if nbytes else None
     _call("kv_attention", L.ntb_kv_attention, c._index, qd, c._desc, td, ld, sd, _pack(output, _QUERY_TYPES[query.dtype]),
-          scale, bool(is_causal), ws.data_ptr(), nbytes)
+          scale, bool(is_causal), ws.data_ptr() if nbytes else None, nbytes)
     return output
 
 

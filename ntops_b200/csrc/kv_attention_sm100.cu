@@ -3,8 +3,8 @@
 //
 // A block owns two tiles of 128 packed rows (row = query * group + head of the group: one key
 // block serves the whole group) and walks its keys in blocks of 128:
-//   warp 1      looks up pages and scales and copies the codes of half a block (64 keys) of K or V
-//               at a time into staging slots with TMA;
+//   warps 1, 3  look up pages and scales and copy the codes of half a block (64 keys) of K (warp 1)
+//               or V (3) at a time into staging slots with TMA;
 //   warps 4-7   widen codes to fp16 (exact) into the swizzled operand tiles, two of K (warps 4, 5) and
 //               two of V (6, 7);
 //   warps 0, 2  issue the products of tile 0 and of tile 1 for half blocks (64 keys) i: S_t(i) = Q_t
@@ -18,6 +18,10 @@
 // to the largest vs so far (ratios are powers of two for what ntb_kv_store writes, so nothing
 // rounds outside fp16's subnormals); softmax multiplies scores by the block's ks, and O is rescaled
 // when vs grows, as when the row maximum does (only past 2^8, as P <= 2^8 fits fp16).
+//
+// Where a block has 128 rows or fewer, both tiles hold these rows, tile 0 takes the even blocks of
+// keys and tile 1 the odd ones (a "shared" tile below), each from a stage of its own, and tile 0
+// joins the two through shared memory.
 //
 // What bounds it: the softmax warps' chain, ~4100 cycles a block of keys for 2048 of products and 2048
 // of exponentials (2 x 128 x 128 on a 16-per-clock unit): 2048 queries a row over 8192 and 6144 tokens
@@ -41,7 +45,7 @@ constexpr int kThreads = 512;
 constexpr int kMmaWarp = 0, kTmaWarp = 1, kConvBase = 4, kSoftBase = 8;  // warps 0 and 2 issue tiles 0 and 1
 constexpr float kRescaleThreshold = 8.f;
 constexpr int kHalf = 64;       // keys of a staging slot
-constexpr int kInfo = 4;        // blocks whose scales are kept: see info_full below
+constexpr int kInfo = 8;        // blocks whose scales are kept: see info_full below
 // TMEM columns: S_t's buffer b at 128 t + 64 b (P over its first 32), O_t at 256 + 128 t.
 constexpr uint32_t kSCol = 0, kOCol = 256;
 
@@ -57,8 +61,8 @@ struct Smem {
   static constexpr int SK = V + 2 * TILE;        // 2 slots: the halves of a block
   static constexpr int SV = SK + 2 * SLOT;
   static constexpr int INFO = SV + 2 * SLOT;     // kInfo x 80 bytes
-  static constexpr int BAR = INFO + 512;
-  static constexpr int TOTAL = BAR + 320 + 1024;
+  static constexpr int BAR = INFO + 640;
+  static constexpr int TOTAL = BAR + 384 + 1024;
   static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -66,11 +70,10 @@ struct Smem {
 struct Info {
   float kr[8], vr[8];
   float kref;    // scores carry the ks / kref of their keys
-  float vfac;    // O's factor before this block: the previous vref over this one's
-  float vref;
+  float vref;    // the values carry vs / vref; never falls
   uint32_t holes;  // bit g: group g has no page (or no key)
 };
-static_assert(sizeof(Info) * kInfo <= 512, "info ring");
+static_assert(sizeof(Info) * kInfo <= 640, "info ring");
 
 __device__ __forceinline__ float max3f(float a, float b, float c) {
   float r;
@@ -154,6 +157,11 @@ struct Where {
   int b, head, tile, split, splits;
 };
 
+// Whether a tile of 256 rows has at most 128, which its two halves then share.
+__device__ __forceinline__ bool is_shared(const AttnArgs& a, int tile) {
+  return a.rows - tile * kTiles * BLK <= BLK;
+}
+
 // Without cutting: heavy (late) row tiles of all batch rows and heads first.
 __device__ __forceinline__ Where where_is(const AttnArgs& a, int64_t idx) {
   Where w;
@@ -170,59 +178,73 @@ __device__ __forceinline__ Where where_is(const AttnArgs& a, int64_t idx) {
 // too): pieces of at most `target` key blocks, the smallest that gives no more than `blocks`
 // pieces, so that one wave of them is as even as the lengths allow.  One warp derives it from the
 // lengths.  Batch row b has pieces [first(b), first(b + 1)), its segments' splits fastest.
+// A shared tile's block of keys counts half.
 constexpr int kCutRows = 5;  // batch rows a lane holds: 160 rows at most
 struct Cut {
   int units[kCutRows], target;
-  __device__ __forceinline__ Cut(const AttnArgs& a, int blocks) {
-    const int lane = threadIdx.x & 31, segs = a.tiles * a.c.H;
-    int total = 0;
+  int full, shared;  // row tiles of a (batch row, head): ordinary ones, and the last if it is shared
+  int H;
+  __device__ __forceinline__ Cut(const AttnArgs& a, int blocks)
+      : shared(is_shared(a, a.tiles - 1) ? 1 : 0), H(a.c.H) {
+    full = a.tiles - shared;
+    const int lane = threadIdx.x & 31;
+    unsigned sum = 0, half = 0;
 #pragma unroll
     for (int k = 0; k < kCutRows; ++k) {
       const int b = lane + 32 * k;
       units[k] = b < a.nb ? row_units(a, a.b0 + b) : 0;
-      total += units[k];
+      sum += units[k];
+      half += (units[k] + 1) / 2;
     }
-    total = __reduce_add_sync(0xffffffffu, total);
-    target = max(4, (int)quotient((int64_t)total * segs + blocks - 1, blocks));
-    for (int tries = 0; tries < 32 && pieces(a.nb) * segs > blocks; ++tries) target += (target + 7) / 8;
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    half = __reduce_add_sync(0xffffffffu, half);
+    const int64_t total = ((int64_t)sum * full + (int64_t)half * shared) * H;
+    target = max(4, (int)quotient(total + blocks - 1, blocks));
+    for (int tries = 0; tries < 32 && pieces(a.nb) > blocks; ++tries) target += (target + 7) / 8;
   }
+  // pieces of an ordinary and of a shared tile of the lane's k-th batch row
   __device__ __forceinline__ int splits(int k) const { return (units[k] + target - 1) / target; }
-  // pieces of one segment row of the first n batch rows
+  __device__ __forceinline__ int shared_splits(int k) const { return ((units[k] + 1) / 2 + target - 1) / target; }
+  // pieces of the first n batch rows
   __device__ __forceinline__ int pieces(int n) const {
     const int lane = threadIdx.x & 31;
     int s = 0;
 #pragma unroll
     for (int k = 0; k < kCutRows; ++k)
-      if (lane + 32 * k < n) s += splits(k);
+      if (lane + 32 * k < n) s += H * (full * splits(k) + shared * shared_splits(k));
     return __reduce_add_sync(0xffffffffu, s);
   }
-  __device__ __forceinline__ int splits_of(int b) const {  // the same for every lane
-    int s = 0;
+  // the same for every lane: splits in x, shared_splits in y
+  __device__ __forceinline__ int2 splits_of(int b) const {
+    int2 s = make_int2(0, 0);
 #pragma unroll
     for (int k = 0; k < kCutRows; ++k) {
-      const int v = __shfl_sync(0xffffffffu, splits(k), b & 31);
-      if (k == b >> 5) s = v;
+      const int x = __shfl_sync(0xffffffffu, splits(k), b & 31);
+      const int y = __shfl_sync(0xffffffffu, shared_splits(k), b & 31);
+      if (k == b >> 5) s = make_int2(x, y);
     }
     return s;
   }
   // b < 0: there is no such piece
   __device__ __forceinline__ Where at(const AttnArgs& a, int idx) const {
-    const int segs = a.tiles * a.c.H;
     Where w;
     w.b = -1;
     int before = 0;
     for (int b = 0; b < a.nb; ++b) {
-      const int s = splits_of(b), n = s * segs;
-      if (idx < before + n) {
-        const int r = idx - before;
+      const int2 s = splits_of(b);
+      const int n = full * H * s.x;  // ordinary tiles' pieces, before the shared one's
+      if (idx < before + n + shared * H * s.y) {
+        int r = idx - before;
+        const bool sh = r >= n;
+        if (sh) r -= n;
         w.b = a.b0 + b;
-        w.splits = s;
-        w.split = r % s;
-        w.head = r / s % a.c.H;
-        w.tile = r / s / a.c.H;
+        w.splits = sh ? s.y : s.x;
+        w.split = r % w.splits;
+        w.head = r / w.splits % H;
+        w.tile = sh ? full : r / w.splits / H;
         return w;
       }
-      before += n;
+      before += n + shared * H * s.y;
     }
     return w;
   }
@@ -248,12 +270,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* s_full = bars + 17;   // [tile][buffer]
   uint64_t* p_full = bars + 21;   // [tile][buffer]
   uint64_t* pv_done = bars + 25;  // [tile]
-  // [kInfo] scales of block j.  The producer writes entry j once the converters are through K(j - 1)'s
-  // first slot, so they had its tile, so K(j - 3)'s products were done; those of its last half block
-  // were issued after both tiles' P of block j - 4: entry j - 4 is no longer read.
-  uint64_t* info_full = bars + 27;
+  // [kInfo] scales of block j.  A producer writes its part of entry j once the converters have read
+  // the first half of block j - 1, so they wrote blocks j - 2 and j - 3, so the products with the
+  // tiles of j - 4 and j - 5 were done.  Those of K's last half block were issued after P of the same
+  // tile's block before (j - 5 at least; j - 6 and j - 7 of a shared tile): entry j - 8 is no longer
+  // read.
+  uint64_t* info_full = bars + 35;
   uint64_t* done_bar = bars + 31;  // [tile]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 35);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 43);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Info* info = reinterpret_cast<Info*>(sm + S::INFO);
 
@@ -274,7 +298,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int len = row_length(a, w.b), start = row_start(a, w.b, len);
   const int r0 = w.tile * kTiles * BLK;
-  // Key blocks [jb, jb + n) of this block; tile t takes the first n_t of them.
+  const bool shared = is_shared(a, w.tile);
+  // Key blocks [jb, jb + n) of this block; tile t takes the first n_t of them, or every second one
+  // from the t-th on.
   int n_t[kTiles], k_end = 0, all = 0;
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
@@ -294,9 +320,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     n_t[t] = max(min(n_t[t], je) - jb, 0);
     n = max(n, n_t[t]);
   }
+  if (shared) {
+    n_t[0] = (n + 1) / 2;
+    n_t[1] = n / 2;
+  }
 
   if (threadIdx.x == 0) {
-    const uint32_t users = (n_t[0] > 0) + (n_t[1] > 0);  // tiles that release a block's K and V
+    const uint32_t users = shared ? 1 : (n_t[0] > 0) + (n_t[1] > 0);  // tiles that release a block's K and V
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&q_full[i], 128);
       sm100::mbar_init(&done_bar[i], 1);
@@ -314,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::mbar_init(&s_full[i], 1);
       sm100::mbar_init(&p_full[i], 128);
     }
-    for (int i = 0; i < kInfo; ++i) sm100::mbar_init(&info_full[i], 1);
+    for (int i = 0; i < kInfo; ++i) sm100::mbar_init(&info_full[i], 2);
     *abort_flag = 0;
     sm100::fence_mbar_init();
   }
@@ -329,16 +359,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_dependency_launch();
 
   if (warp < kConvBase) {
-    if (warp == kTmaWarp) {
-      // --------------------------------------------------------------- producer ----
-      // lanes 0-7: the block's 8 groups of 16 keys of K; lanes 8-15: of V.  The lane of a box's
-      // first group copies it.
+    if (warp == kTmaWarp || warp == kTmaWarp + 2) {
+      // --------------------------------------------------------------- producers ----
+      // lanes 0-7: the block's 8 groups of 16 keys.  The lane of a box's first group copies it.
+      const bool is_v = warp != kTmaWarp, mine = lane < 8;
       const int grp = lane & 7;
-      const bool is_v = lane >= 8, mine = lane < 16;
       const bool first = mine && (16 * grp) % sa.box == 0;
       const float* scales = (is_v ? a.c.value_scale : a.c.key_scale) + (int64_t)w.head * (is_v ? a.c.vs_h : a.c.ks_h);
       const int64_t s_p = is_v ? a.c.vs_p : a.c.ks_p;
       const int* ids = a.table.ids + (int64_t)w.b * a.table.s_b;
+      const CUtensorMap* map = is_v ? &tv : &tk;
+      uint64_t* full = is_v ? sv_full : sk_full;
+      uint64_t* empty = is_v ? sv_empty : sk_empty;
+      uint8_t* slots = sm + (is_v ? S::SV : S::SK);
       auto page_id = [&](int j) {  // as the table has it
         const int key = (jb + j) * BLK + 16 * grp;
         if (!mine || j >= n || key >= k_end) return -1;
@@ -346,69 +379,60 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto checked = [&](int id) { return (unsigned)id < (unsigned)a.c.P ? id : -1; };
       auto page_scale = [&](int id) { return id < 0 ? 0.f : scales[(int64_t)id * s_p]; };
+      auto token = [&](int j) {  // of this lane's group in its page
+        const int key = (jb + j) * BLK + 16 * grp;
+        return sa.t_shift >= 0 ? key & (a.c.T - 1) : key % a.c.T;
+      };
       // Ids are loaded two blocks ahead, scales one.
       int id0 = checked(page_id(0)), id1 = page_id(1);
-      float sc0 = page_scale(id0), vrun = 1.17549435e-38f;
+      float sc0 = page_scale(id0), ref = 0.f;
       bool ok = true;
-      int staged = 0;  // slots armed so far, in the order K0 K1 V0 V1 of each block
+      int staged = 0;  // slots armed so far
       for (int j = 0; j < n && ok; ++j) {
-        id1 = checked(id1);
-        const float sc1 = page_scale(id1);
-        const int id2 = page_id(j + 2);
-        // the block's reference scales, over lanes 0-7 and 8-15
-        float top = mine ? fabsf(sc0) : 0.f;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float kref = fmaxf(__shfl_sync(0xffffffffu, top, 0), 1.17549435e-38f);
-        const float vold = vrun;
-        vrun = fmaxf(vrun, __shfl_sync(0xffffffffu, top, 8));
-        const uint32_t holes = ~__ballot_sync(0xffffffffu, id0 >= 0) & 0xFFu;
-        Info* I = &info[j % kInfo];
-        bool wrote = false;
-        for (int q = 0; q < 4 && ok; ++q) {
-          const int h = q & 1;
-          const bool v = q >= 2;
-          uint64_t* full = v ? &sv_full[h] : &sk_full[h];
-          uint64_t* empty = v ? &sv_empty[h] : &sk_empty[h];
-          int go = 1;
-          if (lane == 0) go = sm100::mbar_wait(empty, (uint32_t)((j & 1) ^ 1), abort_flag, a.err);
-          ok = __shfl_sync(0xffffffffu, go, 0);
+        const uint32_t there = __ballot_sync(0xffffffffu, id0 >= 0);
+        const uint32_t boxes = __ballot_sync(0xffffffffu, first && id0 >= 0);
+        const int tok = token(j);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          ok = __all_sync(0xffffffffu, sm100::mbar_wait(&empty[h], (uint32_t)((j & 1) ^ 1), abort_flag, a.err));
           if (!ok) break;
-          if (!wrote) {  // K's slots are free: so is the entry
-            if (mine) (is_v ? I->vr : I->kr)[grp] = sc0 / (is_v ? vrun : kref);
+          // Operands that every lane holds, and one elected lane: see elect_one.
+          if (elect_one())
+            sm100::mbar_arrive_expect_tx(&full[h], __popc((boxes >> (4 * h)) & 15u) * (uint32_t)(sa.box * D));
+          for (int g = 0; g < 4; g += sa.box / 16) {
+            const int id = __shfl_sync(0xffffffffu, id0, 4 * h + g), row = __shfl_sync(0xffffffffu, tok, 4 * h + g);
+            if (id >= 0 && elect_one()) sm100::tma_load_4d(slots + h * S::SLOT + g * 16 * D, map, &full[h], 0, row, w.head, id);
+          }
+          ++staged;
+          if (h == 0) {  // the slot was free: so is the entry
+            // the block's reference scale: its own largest for K, the largest so far for V
+            float top = mine ? fabsf(sc0) : 0.f;
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            ref = fmaxf(__shfl_sync(0xffffffffu, top, 0), is_v && j > 0 ? ref : 1.17549435e-38f);
+            Info* I = &info[j % kInfo];
+            if (mine) (is_v ? I->vr : I->kr)[grp] = sc0 / ref;
             if (lane == 0) {
-              I->kref = kref;
-              I->vfac = j == 0 ? 1.f : vold / vrun;
-              I->vref = vrun;
-              I->holes = holes;
+              (is_v ? I->vref : I->kref) = ref;
+              if (!is_v) I->holes = ~there & 0xFFu;
             }
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&info_full[j % kInfo]);
-            wrote = true;
+            id1 = checked(id1);
+            sc0 = page_scale(id1);
           }
-          const bool go_mine = first && is_v == v && (grp >> 2) == h && id0 >= 0;
-          const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, go_mine));
-          if (lane == 0) sm100::mbar_arrive_expect_tx(full, boxes * (uint32_t)(sa.box * D));
-          __syncwarp();
-          if (go_mine) {
-            const int key = (jb + j) * BLK + 16 * grp;
-            sm100::tma_load_4d(sm + (v ? S::SV : S::SK) + h * S::SLOT + (grp & 3) * 16 * D, v ? &tv : &tk, full, 0,
-                               sa.t_shift >= 0 ? key & (a.c.T - 1) : key % a.c.T, w.head, id0);
-          }
-          ++staged;
         }
         id0 = id1;
-        id1 = id2;
-        sc0 = sc1;
+        id1 = page_id(j + 2);
       }
       // every copy has landed before the block's shared memory goes: the last use of each slot
       if (lane == 0)
-        for (int q = 0; q < 4; ++q) {
-          const int uses = (staged + 3 - q) / 4;
-          if (uses > 0) sm100::mbar_wait_unwind(q >= 2 ? &sv_full[q & 1] : &sk_full[q & 1], (uint32_t)((uses - 1) & 1));
+        for (int h = 0; h < 2; ++h) {
+          const int uses = (staged + 1 - h) / 2;
+          if (uses > 0) sm100::mbar_wait_unwind(&full[h], (uint32_t)((uses - 1) & 1));
         }
       __syncwarp();
-    } else if (warp == kMmaWarp || warp == kMmaWarp + 2) {
+    } else {
       // ------------------------------------------------------------ MMA issuers ----
       constexpr uint32_t idesc_qk = sm100::instr_desc(0, false, false, BLK, kHalf);
       constexpr uint32_t idesc_pv = sm100::instr_desc(0, false, true, BLK, D);
@@ -422,11 +446,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t k_lo = sm100::smem_desc_lo(sm100::smem_u32(sm + S::K), 16);
       const uint32_t v_lo = sm100::smem_desc_lo(sm100::smem_u32(sm + S::V), S::SUB);
       const uint32_t s_col = tmem + kSCol + 128u * t, o_col = tmem + kOCol + 128u * t;
+      const int turn = shared ? 1 : 2;  // bit of i that a stage's phase follows
       // S_t(i) = Q_t K^T of half block i; the block's second half releases K.
       auto issue_s = [&](int i) -> bool {
-        const int st = (i >> 1) & 1, b = i & 1;
+        const int st = shared ? t : (i >> 1) & 1, b = i & 1;
         if (b == 0) {
-          if (!sm100::mbar_wait(&k_full[st], (uint32_t)((i >> 2) & 1), abort_flag, a.err)) return false;
+          if (!sm100::mbar_wait(&k_full[st], (uint32_t)((i >> turn) & 1), abort_flag, a.err)) return false;
           sm100::tc_fence_after();
         }
         if (elect_one()) {
@@ -445,8 +470,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // O_t += P_t(i) V, likewise.
       auto issue_pv = [&](int i) -> bool {
-        const int st = (i >> 1) & 1, b = i & 1;
-        if (b == 0 && !sm100::mbar_wait(&v_full[st], (uint32_t)((i >> 2) & 1), abort_flag, a.err)) return false;
+        const int st = shared ? t : (i >> 1) & 1, b = i & 1;
+        if (b == 0 && !sm100::mbar_wait(&v_full[st], (uint32_t)((i >> turn) & 1), abort_flag, a.err)) return false;
         if (!sm100::mbar_wait(&p_full[2 * t + b], (uint32_t)((i >> 1) & 1), abort_flag, a.err)) return false;
         sm100::tc_fence_after();
         if (elect_one()) {
@@ -471,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) sm100::mma_commit(&done_bar[t]);  // every product of this tile
       __syncwarp();
       // blocks that only the other tile still uses: this one has nothing to hold them for
-      for (int j = n_t[t]; ok && j < n; ++j) {
+      for (int j = n_t[t]; ok && !shared && j < n; ++j) {
         const int st = j & 1;
         const uint32_t phase = (uint32_t)((j >> 1) & 1);
         ok = sm100::mbar_wait(&k_full[st], phase, abort_flag, a.err);
@@ -507,10 +532,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int j = 0; ok && j < n; ++j) {
       const int st = j & 1;
-      ok = sm100::mbar_wait(&info_full[j % kInfo], (uint32_t)((j / kInfo) & 1), abort_flag, a.err) &&
-           sm100::mbar_wait(&tile_empty[st], (uint32_t)(((j >> 1) & 1) ^ 1), abort_flag, a.err);
       const Info* I = &info[j % kInfo];
-      const uint32_t holes = I->holes;
+      uint32_t holes = 0;
 #pragma unroll 1
       for (int h = 0; ok && h < 2; ++h) {
         ok = sm100::mbar_wait(&slot_full[h], (uint32_t)(j & 1), abort_flag, a.err);
@@ -521,6 +544,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int s = 0; s < STEPS; ++s)
             c[q][s] = lds16(src + h * S::SLOT + (16 * q + 8 * (s / HALVES)) * D + off[s % HALVES]);
+        // The slot is free as soon as it is read; the codes wait for their tile in registers.
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&slot_empty[h]);
+        if (h == 0) {
+          ok = sm100::mbar_wait(&info_full[j % kInfo], (uint32_t)((j / kInfo) & 1), abort_flag, a.err) &&
+               sm100::mbar_wait(&tile_empty[st], (uint32_t)(((j >> 1) & 1) ^ 1), abort_flag, a.err);
+          if (!ok) break;
+          holes = I->holes;
+        }
         const int g0 = 4 * h + 2 * sub, key0 = (jb + j) * BLK + 16 * g0;
         const float f[2] = {is_v ? I->vr[g0] : I->kr[g0], is_v ? I->vr[g0 + 1] : I->kr[g0 + 1]};
         if (__builtin_expect(((holes >> g0) & 3) || key0 + 32 > k_end, 0)) {  // what is no key may be anything
@@ -549,8 +581,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             sts16(to + out[0], r[0], r[1], r[2], r[3]);
             sts16(to + out[1], r[4], r[5], r[6], r[7]);
           }
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&slot_empty[h]);
       }
       if (ok) {
         fence_async_smem();
@@ -561,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ softmax ----
     const int t = (warp - kSoftBase) >> 2;
     const int wq = warp & 3;                          // TMEM lane quarter
-    const int rt = t * BLK + wq * 32 + lane;          // row in the block's pair of tiles
+    const int rt = (shared ? 0 : t * BLK) + wq * 32 + lane;  // row in the block's pair of tiles
     const int r = r0 + rt;
     const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
     const uint32_t s_col = tmem + kSCol + 128u * t + lane_addr;
@@ -623,8 +653,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t holes = 0;
     bool ok = true;
     for (int i = 0; i < mine; ++i) {
-      const int j = i >> 1, b = i & 1, k0 = (jb + j) * BLK + kHalf * b;
-      float vfac = 1.f;
+      const int b = i & 1, j = shared ? (i & ~1) + t : i >> 1, k0 = (jb + j) * BLK + kHalf * b;
+      float vfac = 1.f;  // O's factor before this block: the previous vref over this one's
       if (b == 0) {
         if (!sm100::mbar_wait(&info_full[j % kInfo], (uint32_t)((j / kInfo) & 1), abort_flag, a.err)) { ok = false; break; }
         const Info* I = &info[j % kInfo];
@@ -632,13 +662,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         // -inf * 0 would be NaN
         sc = rowsc * I->kref;
         if (sc < 1.17549435e-38f) sc = 1.17549435e-38f;
-        vfac = I->vfac;
         holes = I->holes;
-        vref = I->vref;
+        const float v = I->vref;
+        if (v != vref) vfac = vref / v;  // (of no use before the first block)
+        vref = v;
       }
       const uint32_t s_tmem = s_col + 64u * b;
       const bool edge = __any_sync(0xffffffffu, k0 + kHalf - 1 > kmax) || holes != 0;
-      if (!sm100::mbar_wait(&s_full[2 * t + b], (uint32_t)(j & 1), abort_flag, a.err)) { ok = false; break; }
+      if (!sm100::mbar_wait(&s_full[2 * t + b], (uint32_t)((i >> 1) & 1), abort_flag, a.err)) { ok = false; break; }
       sm100::tc_fence_after();
       uint32_t sr[2][32];
       sm100::tmem_ld_32x32b_x32(s_tmem, sr[0]);
@@ -724,10 +755,44 @@ __global__ void __launch_bounds__(kThreads, 1)
     // wait tells neighbouring phases apart by parity alone.
     if (ok && mine > 0) ok = sm100::mbar_wait(&done_bar[t], 0, abort_flag, a.err);
     sm100::tc_fence_after();
-    if (ok) {
+    // A shared tile's second half hands (m, l) and its sums over in what its own products have read.
+    const bool joined = shared && n_t[1] > 0;
+    float2* stats = reinterpret_cast<float2*>(sm + S::Q + S::TILE) + rt;
+    auto handed = [&](int c) {  // channels [32 c, 32 c + 32) of the row, 128 floats apart
+      constexpr int PER = D / 64;
+      return reinterpret_cast<float*>(sm + (c < PER ? S::K : S::V) + S::TILE) + (c % PER) * 32 * BLK + rt;
+    };
+    const bool none = l == 0.f;  // nothing seen (NaN is not 0)
+    if (joined) {
+      if (t == 1 && ok) {
+        *stats = make_float2(m_used, l);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t x[32];
+          sm100::tmem_ld_32x32b_x32(o_tmem + c * 32, x);
+          sm100::tmem_ld_wait();
+          float* h = handed(c);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) h[i * BLK] = none ? 0.f : __uint_as_float(x[i]) * vref;
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the softmax warps
+    }
+    if (ok && !(shared && t == 1)) {
+      float g = vref, g1 = 0.f;  // factors of this tile's sums and of those handed over
+      if (joined) {
+        const float2 s1 = *stats;
+        const float M = fmaxf(m_used, s1.x), ref = M == -INFINITY ? 0.f : M;
+        g1 = exp2f(s1.x - ref);
+        const float g0 = exp2f(m_used - ref);
+        l = l * g0 + s1.y * g1;
+        g *= g0;
+        m_used = M;
+      }
       const bool whole = w.splits == 1;
-      const float f = !whole ? vref : l == 0.f ? 0.f : vref / l;
-      const bool none = l == 0.f;  // nothing seen (NaN is not 0)
+      const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      g *= inv;
+      g1 *= inv;
       float* part = nullptr;
       T* op = nullptr;
       if (r < a.rows) {
@@ -748,16 +813,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           sm100::tmem_ld_32x32b_x32(o_tmem + c * 32, x);
           sm100::tmem_ld_wait();
         }
-        if (mine == 0 || none) {
+        const bool zero = mine == 0 || none;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = 0u;
+        for (int i = 0; i < 32; ++i) x[i] = zero ? 0u : __float_as_uint(__uint_as_float(x[i]) * g);
+        if (joined) {
+          const float* h = handed(c);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(fmaf(h[i * BLK], g1, __uint_as_float(x[i])));
         }
         if (op != nullptr) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             ew::Vec<T, 8> y;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y.v[e] = cvt<T>(__uint_as_float(x[i + e]) * f);
+            for (int e = 0; e < 8; ++e) y.v[e] = cvt<T>(__uint_as_float(x[i + e]));
             if (sa.o_vec) {
               *reinterpret_cast<ew::Vec<T, 8>*>(op + c * 32 + i) = y;
             } else {
@@ -768,9 +837,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (part != nullptr) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(part + c * 32 + i) =
-                make_float4(__uint_as_float(x[i]) * f, __uint_as_float(x[i + 1]) * f, __uint_as_float(x[i + 2]) * f,
-                            __uint_as_float(x[i + 3]) * f);
+            *reinterpret_cast<uint4*>(part + c * 32 + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
         }
       }
     }
@@ -798,7 +865,10 @@ __global__ void __launch_bounds__(128) kv_split_combine(AttnArgs a, int blocks) 
   if (b >= a.nb) return;
   const int tile = seg / a.c.H, head = seg % a.c.H, r = tile * rows + rt;
   if (r >= a.rows) return;
-  const int splits = cut.splits_of(b), first = cut.pieces(b) * segs + seg * splits;
+  const int2 s_of = cut.splits_of(b);
+  const bool shared = tile >= cut.full;
+  const int splits = shared ? s_of.y : s_of.x;
+  const int first = cut.pieces(b) + min(tile, cut.full) * a.c.H * s_of.x + head * splits;
   if (splits == 1) return;  // its block wrote the output
   const int64_t slot = slot_floats(rows, D);
   const float* base = a.part + (int64_t)first * slot;

@@ -39,7 +39,9 @@ namespace {
 constexpr int kConsumers = 4;
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kUnit = 128;            // keys of a unit: 32 a consumer warp
-constexpr float kGrow = 6.f;          // rows rescale when their maximum grows by more (p <= 2^6)
+// p = 2^(score - m): m is set 7 below a row's maximum and follows when that grows 14 above it (p <=
+// 2^14).  So the largest p is 2^7 or more, and those that fp16 begins to lose are under 2^-21 of it.
+constexpr float kTop = 7.f, kGrow = 14.f;
 
 // Four codes -> two fp16 pairs (bytes 0, 1 and 2, 3).
 template <int CODE>
@@ -425,8 +427,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<D, RT>::BLOCKS)) decode_kernel(
         for (int x = 0; x < RT; ++x) {
           float alpha = 1.f;
           if (mb[x] > m[x] + kGrow) {
-            alpha = exp2f(m[x] - mb[x]);  // 0 at the first block that the row sees
-            m[x] = mb[x];
+            alpha = exp2f(m[x] - (mb[x] - kTop));  // 0 at the first block that the row sees
+            m[x] = mb[x] - kTop;
           }
           l[x] *= alpha;
           // O^T's columns are rows 2t and 2t + 1, whose statistics lanes 8t and 8t + 4 hold

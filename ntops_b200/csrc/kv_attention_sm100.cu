@@ -17,17 +17,18 @@
 // Page scales: within a block keys are widened relative to the block's largest ks, values relative
 // to the largest vs so far (ratios are powers of two for what ntb_kv_store writes, so nothing
 // rounds outside fp16's subnormals); softmax multiplies scores by the block's ks, and O is rescaled
-// when vs grows, as when the row maximum does (only past 2^8, as P <= 2^8 fits fp16).
+// when vs grows, as when the row maximum does (see kTop).
 //
 // Where a block has 128 rows or fewer, both tiles hold these rows, tile 0 takes the even blocks of
 // keys and tile 1 the odd ones (a "shared" tile below), each from a stage of its own, and tile 0
 // joins the two through shared memory.
 //
-// What bounds it: the softmax warps' chain, ~4100 cycles a block of keys for 2048 of products and 2048
+// What bounds it: the softmax warps' chain, ~4000 cycles a block of keys for 2048 of products and 2048
 // of exponentials (2 x 128 x 128 on a 16-per-clock unit): 2048 queries a row over 8192 and 6144 tokens
-// (32 heads, 8 kv heads of 128) take 468 us, 880 TFLOP/s.  Where one wave of blocks would leave SMs
+// (32 heads, 8 kv heads of 128) take 459 us, 898 TFLOP/s.  Where one wave of blocks would leave SMs
 // idle, several blocks share a tile's keys, cut evenly by the lengths, and kv_split_combine joins
-// them.
+// them.  A shared tile's chain is K's and V's way from staging slot to operand tile instead: 128 rows
+// over 8 x 16384 keys take 124 us, 181 before tiles were shared.
 #include <algorithm>
 #include <type_traits>
 
@@ -43,7 +44,9 @@ constexpr int BLK = 128;
 constexpr int kTiles = 2;
 constexpr int kThreads = 512;
 constexpr int kMmaWarp = 0, kTmaWarp = 1, kConvBase = 4, kSoftBase = 8;  // warps 0 and 2 issue tiles 0 and 1
-constexpr float kRescaleThreshold = 8.f;
+// P = 2^(score - m_used): up to 2^15 before a larger maximum makes m_used follow, to 7 below it, so
+// that the largest P of a row is 2^7 or more and those that fp16 begins to lose are under 2^-21 of it.
+constexpr float kTop = 7.f, kRescaleThreshold = 15.f;
 constexpr int kHalf = 64;       // keys of a staging slot
 constexpr int kInfo = 8;        // blocks whose scales are kept: see info_full below
 // TMEM columns: S_t's buffer b at 128 t + 64 b (P over its first 32), O_t at 256 + 128 t.
@@ -178,7 +181,8 @@ __device__ __forceinline__ Where where_is(const AttnArgs& a, int64_t idx) {
 // too): pieces of at most `target` key blocks, the smallest that gives no more than `blocks`
 // pieces, so that one wave of them is as even as the lengths allow.  One warp derives it from the
 // lengths.  Batch row b has pieces [first(b), first(b + 1)), its segments' splits fastest.
-// A shared tile's block of keys counts half.
+// A shared tile's block of keys counts three quarters (measured: 126 us against 179 us for 128 and 256
+// rows over 8 x 16384 keys).
 constexpr int kCutRows = 5;  // batch rows a lane holds: 160 rows at most
 struct Cut {
   int units[kCutRows], target;
@@ -188,23 +192,24 @@ struct Cut {
       : shared(is_shared(a, a.tiles - 1) ? 1 : 0), H(a.c.H) {
     full = a.tiles - shared;
     const int lane = threadIdx.x & 31;
-    unsigned sum = 0, half = 0;
+    unsigned sum = 0, part = 0;
 #pragma unroll
     for (int k = 0; k < kCutRows; ++k) {
       const int b = lane + 32 * k;
       units[k] = b < a.nb ? row_units(a, a.b0 + b) : 0;
       sum += units[k];
-      half += (units[k] + 1) / 2;
+      part += shared_units(units[k]);
     }
     sum = __reduce_add_sync(0xffffffffu, sum);
-    half = __reduce_add_sync(0xffffffffu, half);
-    const int64_t total = ((int64_t)sum * full + (int64_t)half * shared) * H;
+    part = __reduce_add_sync(0xffffffffu, part);
+    const int64_t total = ((int64_t)sum * full + (int64_t)part * shared) * H;
     target = max(4, (int)quotient(total + blocks - 1, blocks));
     for (int tries = 0; tries < 32 && pieces(a.nb) > blocks; ++tries) target += (target + 7) / 8;
   }
+  __device__ static __forceinline__ int shared_units(int u) { return u - u / 4; }
   // pieces of an ordinary and of a shared tile of the lane's k-th batch row
   __device__ __forceinline__ int splits(int k) const { return (units[k] + target - 1) / target; }
-  __device__ __forceinline__ int shared_splits(int k) const { return ((units[k] + 1) / 2 + target - 1) / target; }
+  __device__ __forceinline__ int shared_splits(int k) const { return (shared_units(units[k]) + target - 1) / target; }
   // pieces of the first n batch rows
   __device__ __forceinline__ int pieces(int n) const {
     const int lane = threadIdx.x & 31;
@@ -563,24 +568,31 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (((holes >> (g0 + q)) & 1) || key0 + 16 * q + 8 * (s / HALVES) + row >= k_end)
                 c[q][s] = make_uint4(0, 0, 0, 0);
         }
+        const uint32_t to0 = dst + st * S::TILE + 64 * h * 128;
+        auto write = [&](auto scaled) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+          for (int q = 0; q < 2; ++q) {
+            const __half2 f2 = __float2half2_rn(((holes >> (g0 + q)) & 1) ? 0.f : f[q]);
 #pragma unroll
-          for (int s = 0; s < STEPS; ++s) {
-            uint32_t r[8];
-            widen4<CODE>(c[q][s].x, r[0], r[1]);
-            widen4<CODE>(c[q][s].y, r[2], r[3]);
-            widen4<CODE>(c[q][s].z, r[4], r[5]);
-            widen4<CODE>(c[q][s].w, r[6], r[7]);
-            if (f[q] != 1.f) {  // the same for the whole warp
-              const __half2 f2 = __float2half2_rn(((holes >> (g0 + q)) & 1) ? 0.f : f[q]);
+            for (int s = 0; s < STEPS; ++s) {
+              uint32_t r[8];
+              widen4<CODE>(c[q][s].x, r[0], r[1]);
+              widen4<CODE>(c[q][s].y, r[2], r[3]);
+              widen4<CODE>(c[q][s].z, r[4], r[5]);
+              widen4<CODE>(c[q][s].w, r[6], r[7]);
+              if constexpr (decltype(scaled)::value) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) r[i] = mul2(r[i], f2);
+                for (int i = 0; i < 8; ++i) r[i] = mul2(r[i], f2);
+              }
+              const uint32_t to = to0 + (s % HALVES) * S::SUB + (16 * q + 8 * (s / HALVES)) * 128;
+              sts16(to + out[0], r[0], r[1], r[2], r[3]);
+              sts16(to + out[1], r[4], r[5], r[6], r[7]);
             }
-            const uint32_t to = dst + st * S::TILE + (s % HALVES) * S::SUB + (64 * h + 16 * q + 8 * (s / HALVES)) * 128;
-            sts16(to + out[0], r[0], r[1], r[2], r[3]);
-            sts16(to + out[1], r[4], r[5], r[6], r[7]);
           }
+        };
+        // (the same for the whole warp; a branch at every step would keep the steps from overlapping)
+        if (f[0] == 1.f && f[1] == 1.f) write(std::false_type());
+        else write(std::true_type());
       }
       if (ok) {
         fence_async_smem();
@@ -703,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float m_blk = fmaxf(max3f(mx4[0], mx4[1], mx4[2]), mx4[3]) * sc;
       const bool grow = m_blk > m_used + kRescaleThreshold;
       const float m_prev = m_used;
-      if (grow) m_used = m_blk;
+      if (grow) m_used = m_blk - kTop;
       const float m_ref = m_used == -INFINITY ? 0.f : m_used;
       const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(-m_ref, -m_ref);
 #pragma unroll
@@ -722,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float alpha = 1.f;
       if (__builtin_expect(__any_sync(0xffffffffu, (grow || vfac != 1.f) && i > 0), 0)) {
-        alpha = grow ? exp2f(m_prev - m_blk) : 1.f;
+        alpha = grow ? exp2f(m_prev - m_used) : 1.f;
         // PV_t(i-1) must be complete (PV_t(i-2) is: S_t(i) was issued after it).
         if (!sm100::mbar_wait(&pv_done[t], (uint32_t)((i - 1) & 1), abort_flag, a.err)) { ok = false; break; }
         sm100::tc_fence_after();

@@ -113,6 +113,23 @@ def test_attention(lengths, sq, hq, hkv, d, page, code, dtype, causal):
     _check_attention(got, q, cache, 1, table, n, scale, causal)
 
 
+@pytest.mark.parametrize("sq,group,d,code,dtype", [
+    (33, 1, 128, E4M3, BF16), (32, 4, 128, I8, F16), (129, 1, 64, E4M3, F16), (96, 4, 128, E4M3, BF16), (64, 2, 64, I8, BF16),
+])
+@pytest.mark.parametrize("b", [3, 20])  # fewer segments than multiprocessors (keys are cut) and more
+def test_attention_last_rows_share_the_keys(b, sq, group, d, code, dtype):
+    """Up to 128 rows, alone or after whole tiles of 256: odd and even numbers of key blocks, values'
+    scales that grow from page to page, rows with none or one of the blocks."""
+    page, hkv = 32, 8
+    lengths = [(1000, 0, 257, 128, 1, 640, 129)[i % 7] for i in range(b)]
+    cache = _random_cache(1, sum(-(-n // page) for n in lengths) + 1, hkv, page, d, code, scale_lo=-9, scale_hi=-3)
+    table = _table(lengths, page, cache.key.shape[1])
+    q = torch.randn(b, hkv * group, sq, d).to(dtype)
+    n = torch.tensor(lengths, dtype=torch.int32)
+    got = kc.attention(q.to(DEV), cache.layer(0), table.to(DEV), n.to(DEV), is_causal=b == 3)
+    _check_attention(got, q, cache, 0, table, n, 1 / math.sqrt(d), b == 3)
+
+
 @pytest.mark.parametrize("dtype,d,sq", [(BF16, 128, 1), (F16, 64, 3), (F32, 64, 2), (BF16, 128, 40)])
 def test_attention_rows_that_see_nothing(dtype, d, sq):
     """Empty rows, rows of holes only, and queries before the first key give zeros."""

@@ -113,10 +113,13 @@ def test_attention(lengths, sq, hq, hkv, d, page, code, dtype, causal):
     _check_attention(got, q, cache, 1, table, n, scale, causal)
 
 
-@pytest.mark.parametrize("sq,group,d,code,dtype", [
-    (33, 1, 128, E4M3, BF16), (32, 4, 128, I8, F16), (129, 1, 64, E4M3, F16), (96, 4, 128, E4M3, BF16), (64, 2, 64, I8, BF16),
+@pytest.mark.parametrize("b,sq,group,d,code,dtype", [
+    # fewer segments than multiprocessors: keys are cut
+    (3, 33, 1, 128, E4M3, BF16), (3, 32, 4, 128, I8, F16), (3, 129, 1, 64, E4M3, F16), (3, 96, 4, 128, E4M3, BF16),
+    (3, 64, 2, 64, I8, BF16),
+    # and more
+    (20, 33, 1, 128, E4M3, BF16), (20, 17, 2, 64, I8, F16), (10, 257, 1, 128, I8, BF16),
 ])
-@pytest.mark.parametrize("b", [3, 20])  # fewer segments than multiprocessors (keys are cut) and more
 def test_attention_last_rows_share_the_keys(b, sq, group, d, code, dtype):
     """Up to 128 rows, alone or after whole tiles of 256: odd and even numbers of key blocks, values'
     scales that grow from page to page, rows with none or one of the blocks."""

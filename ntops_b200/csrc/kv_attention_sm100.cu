@@ -28,7 +28,7 @@
 // (32 heads, 8 kv heads of 128) take 459 us, 898 TFLOP/s.  Where one wave of blocks would leave SMs
 // idle, several blocks share a tile's keys, cut evenly by the lengths, and kv_split_combine joins
 // them.  A shared tile's chain is K's and V's way from staging slot to operand tile instead: 128 rows
-// over 8 x 16384 keys take 124 us, 181 before tiles were shared.
+// over 8 x 16384 keys take 124 us, 153 with all blocks in one tile.
 #include <algorithm>
 #include <type_traits>
 
@@ -160,7 +160,10 @@ struct Where {
   int b, head, tile, split, splits;
 };
 
-// Whether a tile of 256 rows has at most 128, which its two halves then share.
+// Whether a tile of 256 rows has at most 128, which its two halves then share if there are kShareMin
+// blocks of keys: 48 rows over 16384 keys, cut into pieces of 8 blocks, take 30 us shared and 35 not;
+// over 4096 keys, in pieces of 5 and 4, 22.7 and 20.8, as the join then costs more than it saves.
+constexpr int kShareMin = 8;
 __device__ __forceinline__ bool is_shared(const AttnArgs& a, int tile) {
   return a.rows - tile * kTiles * BLK <= BLK;
 }
@@ -181,7 +184,7 @@ __device__ __forceinline__ Where where_is(const AttnArgs& a, int64_t idx) {
 // too): pieces of at most `target` key blocks, the smallest that gives no more than `blocks`
 // pieces, so that one wave of them is as even as the lengths allow.  One warp derives it from the
 // lengths.  Batch row b has pieces [first(b), first(b + 1)), its segments' splits fastest.
-// A shared tile's block of keys counts three quarters (measured: 126 us against 179 us for 128 and 256
+// A shared tile's block of keys counts three quarters (measured: 124 us against 173 us for 128 and 256
 // rows over 8 x 16384 keys).
 constexpr int kCutRows = 5;  // batch rows a lane holds: 160 rows at most
 struct Cut {
@@ -203,7 +206,7 @@ struct Cut {
     sum = __reduce_add_sync(0xffffffffu, sum);
     part = __reduce_add_sync(0xffffffffu, part);
     const int64_t total = ((int64_t)sum * full + (int64_t)part * shared) * H;
-    target = max(4, (int)quotient(total + blocks - 1, blocks));
+    target = max(full > 0 ? 4 : 3, (int)quotient(total + blocks - 1, blocks));
     for (int tries = 0; tries < 32 && pieces(a.nb) > blocks; ++tries) target += (target + 7) / 8;
   }
   __device__ static __forceinline__ int shared_units(int u) { return u - u / 4; }
@@ -303,7 +306,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int len = row_length(a, w.b), start = row_start(a, w.b, len);
   const int r0 = w.tile * kTiles * BLK;
-  const bool shared = is_shared(a, w.tile);
   // Key blocks [jb, jb + n) of this block; tile t takes the first n_t of them, or every second one
   // from the t-th on.
   int n_t[kTiles], k_end = 0, all = 0;
@@ -325,6 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     n_t[t] = max(min(n_t[t], je) - jb, 0);
     n = max(n, n_t[t]);
   }
+  const bool shared = is_shared(a, w.tile) && n >= kShareMin;
   if (shared) {
     n_t[0] = (n + 1) / 2;
     n_t[1] = n / 2;

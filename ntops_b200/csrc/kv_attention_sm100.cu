@@ -25,7 +25,7 @@
 //
 // What bounds it: the softmax warps' chain, ~4000 cycles a block of keys for 2048 of products and 2048
 // of exponentials (2 x 128 x 128 on a 16-per-clock unit): 2048 queries a row over 8192 and 6144 tokens
-// (32 heads, 8 kv heads of 128) take 459 us, 898 TFLOP/s.  Where one wave of blocks would leave SMs
+// (32 heads, 8 kv heads of 128) take 463 us, 890 TFLOP/s.  Where one wave of blocks would leave SMs
 // idle, several blocks share a tile's keys, cut evenly by the lengths, and kv_split_combine joins
 // them.  A shared tile's chain is K's and V's way from staging slot to operand tile instead: 128 rows
 // over 8 x 16384 keys take 124 us, 153 with all blocks in one tile.
